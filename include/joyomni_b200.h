@@ -233,6 +233,86 @@ int jo_fp8_scaled_mm_scatter(const void* mat_a, const void* mat_b, const float* 
                              int64_t tok0, int64_t dst_tokens, void* stream);
 
 /*
+ * Paged K/V cache and attention over requests of different lengths (no
+ * reference counterpart: the reference keeps one dense K/V buffer per session
+ * and attends without a mask).  A cache is [num_blocks, page_size, kv_heads,
+ * head_dim]; token position pos of request b lives in slot
+ * block_tables[b, pos / page_size] * page_size + pos % page_size.
+ *
+ * jo_paged_layout: the step's block tables, slots and offsets from request
+ * lengths, in one launch.  For request b with cached_lens[b] tokens in the
+ * cache and new_lens[b] new ones (negative lengths count as 0):
+ *   query_starts[b] = sum of the earlier requests' new tokens (batch + 1 entries),
+ *   kv_lens[b] = cached_lens[b] + new_lens[b];
+ *   the blocks it needs beyond the ones it holds are taken from the front of
+ *   free_blocks in request order and stored in its row of block_tables;
+ *   every new token's position and slot follow, request after request.
+ * blocks_needed: how many free blocks the step takes.  Where the list (num_free
+ * entries) or the table (table_width) is too short, the slot (and the table
+ * entry) is -1.  Places after the last request up to num_tokens have slot -1
+ * and position 0.  num_tokens must be at least the sum of the new lengths:
+ * tokens past it are left out, with the blocks that start at them.
+ * table_stride: elements between table rows.
+ */
+int jo_paged_layout(const int32_t* cached_lens, const int32_t* new_lens, int32_t* block_tables,
+                    const int32_t* free_blocks, int64_t batch, int64_t table_width, int64_t table_stride,
+                    int64_t num_free, int64_t page_size, int64_t num_tokens, int32_t* query_starts, int32_t* kv_lens,
+                    int64_t* slots, int32_t* positions, int32_t* blocks_needed, void* stream);
+
+/*
+ * Stores rows of key and value [tokens, kv_heads, head_dim] into their slots of
+ * the caches; rows whose slot is negative or past the cache are left out.
+ * k_strides, v_strides: token and head strides; kc_strides, vc_strides: block,
+ * token and head strides (elements, multiples of 8, rows of head_dim elements
+ * dense).  head_dim % 8 == 0; dtype JO_DTYPE_BF16/F16; 16-byte aligned tensors.
+ */
+int jo_paged_kv_write(const void* key, const void* value, void* key_cache, void* value_cache, const int64_t* slots,
+                      int64_t tokens, int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t page_size,
+                      const int64_t* k_strides, const int64_t* v_strides, const int64_t* kc_strides,
+                      const int64_t* vc_strides, int dtype, void* stream);
+
+/*
+ * Attention of new tokens (one or a chunk a request) over a paged cache:
+ * out = softmax(scale * q k^T) v.  Request b has the query rows
+ * query_starts[b] .. query_starts[b + 1] (n of them) of q [tokens, heads,
+ * head_dim] and the keys 0 .. kv_lens[b] of its blocks, the new tokens' own
+ * among them; row i sees keys 0 .. kv_lens[b] - n + i (causal != 0) or all.  A
+ * row that sees no key is zero; rows of no request are not written.  Query
+ * head h reads key head h / (heads / kv_heads).  Places of a block that no
+ * token holds are never used, whatever they contain; a table entry outside the
+ * cache reads as zeros; kv_lens past table_width pages are cut there.
+ * max_query_len: the largest number of new tokens of a request, as far as the
+ * host knows it (it only chooses the kernels; any value gives the result).
+ * head_dim 64 or 128; dtype JO_DTYPE_BF16/F16; page_size % 16 == 0;
+ * heads / kv_heads <= 128.  Strides (elements, multiples of 8): q, out: token
+ * and head; caches: block, token and head.  workspace: at least
+ * jo_varlen_attention_workspace bytes, 16-byte aligned, used by one call at a
+ * time.
+ */
+int jo_paged_attention(const void* q, const void* key_cache, const void* value_cache, const int32_t* block_tables,
+                       const int32_t* query_starts, const int32_t* kv_lens, void* out, int64_t tokens, int64_t batch,
+                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t page_size,
+                       int64_t table_width, int64_t table_stride, const int64_t* q_strides, const int64_t* kc_strides,
+                       const int64_t* vc_strides, const int64_t* o_strides, int causal, float scale,
+                       int64_t max_query_len, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention of whole packed prompts: request b is rows seq_starts[b] ..
+ * seq_starts[b + 1] of q [tokens, heads, head_dim] and of k, v [tokens,
+ * kv_heads, head_dim]; row i sees keys 0 .. i (causal != 0) or all of its own
+ * request.  Everything else as jo_paged_attention; strides: token and head.
+ */
+int jo_prompt_attention(const void* q, const void* k, const void* v, const int32_t* seq_starts, void* out,
+                        int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                        const int64_t* o_strides, int causal, float scale, int dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that the two calls above need for these sizes (the
+ * partial results of work that is split along the keys). */
+int jo_varlen_attention_workspace(int64_t tokens, int64_t heads, int64_t head_dim, int64_t* bytes);
+
+/*
  * Peer-memory plumbing (legacy CUDA IPC, no multicast objects) for the
  * exchange above.  jo_ipc_get_handle writes the 64-byte handle of the
  * allocation holding dev_ptr and the byte offset of dev_ptr in it;

@@ -15,6 +15,8 @@ Extra entry points with no reference counterpart:
   * ``attention``               — tcgen05 attention forward over NHD bf16 tensors
   * ``attention_scatter``       — the same, output rows stored to the ranks owning them
     (the reference model's external FA4 / SDPA call, dit.py:150-178);
+  * ``paged_layout``, ``paged_kv_write``, ``paged_attention``, ``prompt_attention`` —
+    a paged K/V cache and attention over requests of different lengths (paged.py);
   * broadcast modulation in ``fused_norm_scale_shift``: scale/shift given as an
     expanded view (row stride 0) are read in place instead of being materialised.
 """
@@ -43,6 +45,12 @@ __all__ = [
     "attention",
     "attention_scatter",
     "rope_apply",
+    "PagedLayout",
+    "paged_layout",
+    "paged_kv_write",
+    "paged_attention",
+    "prompt_attention",
+    "varlen_attention_workspace",
 ]
 
 _DT = {torch.float32: _lib.JO_DTYPE_F32, torch.float16: _lib.JO_DTYPE_F16, torch.bfloat16: _lib.JO_DTYPE_BF16}
@@ -527,4 +535,6 @@ def attention_scatter(query, key, value, dst_ptrs, seg_start, head0, total_heads
                                            total_heads * Dh, dst_tokens, sc, _lib.JO_DTYPE_BF16, st))
 
 
+from .paged import (PagedLayout, paged_attention, paged_kv_write, paged_layout, prompt_attention,  # noqa: E402
+                    varlen_attention_workspace)
 from . import _torch_ops  # noqa: E402,F401  (registers torch.ops.joyomni_ops.*)
