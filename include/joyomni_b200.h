@@ -312,6 +312,10 @@ int jo_prompt_attention(const void* q, const void* k, const void* v, const int32
  * partial results of work that is split along the keys). */
 int jo_varlen_attention_workspace(int64_t tokens, int64_t heads, int64_t head_dim, int64_t* bytes);
 
+/* Diagnostic: fault code left by a wait of the two calls above that timed out
+ * (0 = none); reset != 0 clears it.  Synchronous. */
+int jo_varlen_attention_last_fault(int reset);
+
 /*
  * Peer-memory plumbing (legacy CUDA IPC, no multicast objects) for the
  * exchange above.  jo_ipc_get_handle writes the 64-byte handle of the

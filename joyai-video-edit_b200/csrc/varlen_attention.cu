@@ -6,100 +6,805 @@
 // Request b has the query rows query_starts[b] .. query_starts[b + 1] and
 // kv_len keys; row i of its n rows sees keys 0 .. kv_len - n + i (causal) or
 // all of them.  A row that sees no key is zero.
+//
+// Organisation of tile_kernel (one block per SM, 384 threads).  The `group`
+// query heads that read one key head are rows of one tile: row r of a tile is
+// token r / group, head r % group, so K and V are read once for all of them.
+// An item is (request, key head, 256 rows as two 128-row tiles); its unit of
+// work is one step over 128 keys.  The units of all items, laid end to end, are
+// cut into one equal range per block, so that ragged lengths and single long
+// requests fill the machine alike; an item that a cut divides leaves partial
+// results (maximum, sum, unnormalised row) that join_kernel adds up in the order
+// of the keys, so results do not depend on timing.
+//   warp 8       TMA producer: Q tiles of an item, K and V of every step (pages
+//                looked up in the block table, one copy per run of a page)
+//   warp 9       MMA issuer: S_t = Q_t K^T, O_t += P_t V on tcgen05, in the order
+//                PV0 QK0' PV1 QK1' so that the softmax of one tile overlaps the
+//                MMAs of the other, across items too
+//   warps 10-11  look after V in steps where some row does not see every key:
+//                rows past the last visible key are zeroed (a product with P = 0
+//                would turn a NaN there into NaN), and a value row that only some
+//                rows may see is searched for NaN and infinities
+//   warps 0-7    softmax: one thread per row, P over S in tensor memory
+// The running maximum only moves when it grows by more than 2^8, so most steps
+// leave O alone.
 #include <math.h>
 
-#include "jo_common.cuh"
+#include "sm100_async.cuh"
+#include "varlen_attention.cuh"
 
 namespace jo {
 namespace vattn {
 
-// What both forms share.  Strides in elements.
-struct Params {
-  const void* q;
-  const void* k;
-  const void* v;
-  void* out;
-  const int32_t* starts;        // [batch + 1]
-  const int32_t* kv_lens;       // [batch], NULL: as many keys as rows (packed prompts)
-  const int32_t* table;         // [batch, width], NULL: keys packed like the queries
-  int64_t q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_ts, o_hs, table_stride;
-  int tokens, batch, heads, group, head_dim, num_blocks, page, width, causal;
-  float scale;
+using namespace sm100;
+
+constexpr int kRows = 128;               // rows of a tile
+constexpr int kKeys = 128;               // keys of a step
+constexpr int kThreads = 384;
+constexpr int kMaxBlocks = 256;          // blocks of the tile kernel: one per SM
+constexpr int kScan = 512;               // requests of one scan of the lengths
+// A cut closer than this many steps to an item's edge moves to the edge: a
+// shorter piece would cost more to join than to compute.
+constexpr int kMinPiece = 3;
+
+__device__ int g_fault = 0;
+
+// ------------------------------------------------------------ work ranges --
+// Where block c's range of units lies.
+struct Range {
+  int b, h, qt, tile;                    // first unit; tile may be its item's end
+  long long units;
 };
 
-// Rows [first, first + n) and keys of request b; lengths are device data and
-// are clamped to what the tensors hold.
-struct Request {
-  int first, n, keys;
-};
-__device__ __forceinline__ Request request(const Params& p, int b) {
-  Request r;
-  r.first = min(max(p.starts[b], 0), p.tokens);
-  r.n = min(max(p.starts[b + 1], r.first), p.tokens) - r.first;
-  r.keys = p.kv_lens ? (int)min((int64_t)max(p.kv_lens[b], 0), (int64_t)p.width * p.page) : r.n;
-  return r;
+__device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
+// Steps of item qt: at least one, so that rows that see no key are written too.
+__device__ __forceinline__ int item_units(const Params& p, const Request& r, int qt, int tpt) {
+  const int last = min(r.n, (qt + 1) * 2 * tpt) - 1;
+  return max(1, div_up(visible(p, r, last), kKeys));
 }
 
-// One warp per (token, head); D / 32 dimensions in each lane.
+struct ScanSpace {
+  int first[kScan], n[kScan], keys[kScan];
+  long long before[kScan + 1];           // units before each request of the scan
+  Range cut[2];
+  long long at[2];
+};
+
+// Range of block c of C.  All threads of the block take part.
+__device__ void find_range(const Params& p, int tpt, int c, int C, ScanSpace& s, Range& range) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunks = div_up(p.batch, kScan);
+  long long total = 0, target = 0;
+  // First time round: the number of units.  Second: the places of the cuts.
+  for (int round = 0; round < 2; ++round) {
+    if (round == 1) {
+      target = warp < 2 ? total / C * (c + warp) + total % C * (c + warp) / C : 0;
+      if (warp < 2 && lane == 0) {
+        s.cut[warp] = Range{p.batch, 0, 0, 0, 0};
+        s.at[warp] = total;
+      }
+      __syncwarp();
+    }
+    long long base = 0;
+    for (int ch = 0; ch < chunks; ++ch) {
+      const int cnt = min(kScan, p.batch - ch * kScan);
+      if (round == 0 || chunks > 1) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < cnt; i += kThreads) {
+          const Request r = request(p, ch * kScan + i);
+          s.first[i] = r.first;
+          s.n[i] = r.n;
+          s.keys[i] = r.keys;
+        }
+        __syncthreads();
+        for (int i = warp; i < cnt; i += kThreads / 32) {
+          const Request r{s.first[i], s.n[i], s.keys[i]};
+          const int nq = div_up(r.n, 2 * tpt);
+          long long u = 0;
+          for (int q = lane; q < nq; q += 32) u += item_units(p, r, q, tpt);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+          if (lane == 0) s.before[i + 1] = u * p.kv_heads;
+        }
+        __syncthreads();
+        if (warp == 0) {
+          constexpr int E = kScan / 32;
+          long long mine = 0;
+          for (int i = lane * E; i < min(cnt, lane * E + E); ++i) mine += s.before[i + 1];
+          long long inc = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
+          }
+          long long run = inc - mine;
+          if (lane == 0) s.before[0] = 0;
+          for (int i = lane * E; i < min(cnt, lane * E + E); ++i) {
+            run += s.before[i + 1];
+            s.before[i + 1] = run;
+          }
+        }
+        __syncthreads();
+      }
+      const long long sum = s.before[cnt];
+      if (round == 1 && warp < 2 && target >= base && target < base + sum) {
+        const long long rel = target - base;
+        int a = 0, e = cnt;              // last request that begins at or before rel
+        while (e - a > 1) {
+          const int mid = (a + e) >> 1;
+          if (s.before[mid] <= rel) a = mid; else e = mid;
+        }
+        const Request r{s.first[a], s.n[a], s.keys[a]};
+        const long long per_head = (s.before[a + 1] - s.before[a]) / p.kv_heads;
+        const long long in_req = rel - s.before[a];
+        const int h = (int)(in_req / per_head);
+        long long off = in_req - h * per_head;
+        const int nq = div_up(r.n, 2 * tpt);
+        for (int q0 = 0; q0 < nq; q0 += 32) {
+          const int q = q0 + lane;
+          const long long u = q < nq ? item_units(p, r, q, tpt) : 0;
+          long long inc = u;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
+          }
+          const unsigned hit = __ballot_sync(0xffffffffu, inc > off);
+          if (hit) {
+            if (lane == __ffs(hit) - 1) {
+              long long tile = off - (inc - u), at = target;
+              if (tile < kMinPiece) {
+                at -= tile;
+                tile = 0;
+              } else if (u - tile < kMinPiece) {
+                at += u - tile;
+                tile = u;
+              }
+              s.cut[warp] = Range{ch * kScan + a, h, q, (int)tile, 0};
+              s.at[warp] = at;
+            }
+            break;
+          }
+          off -= __shfl_sync(0xffffffffu, inc, 31);
+        }
+      }
+      base += sum;
+    }
+    total = base;
+  }
+  __syncthreads();
+  range = s.cut[0];
+  range.units = s.at[1] - s.at[0];
+}
+
+// One block's stretch of one item.
+struct Piece {
+  int b, h, qt;
+  Request r;
+  int a, e;                              // steps [a, e) of the item's `units`
+  int units;
+  int end[2];                            // tile t takes part in steps [a, end[t])
+  int edge;                              // first step in which some row does not see every key
+};
+
+// Walks a range piece by piece; every role of a block walks it for itself.
+struct Walk {
+  const Params& p;
+  int tpt, b, h, qt, tile, nq;
+  long long left;
+  Request r;
+  __device__ Walk(const Params& p_, int tpt_, const Range& g)
+      : p(p_), tpt(tpt_), b(g.b), h(g.h), qt(g.qt), tile(g.tile), left(g.units) {
+    if (left > 0) load();
+  }
+  __device__ void load() {
+    r = request(p, b);
+    nq = div_up(r.n, 2 * tpt);
+  }
+  __device__ void advance() {
+    tile = 0;
+    if (++qt < nq) return;
+    qt = 0;
+    if (++h < p.kv_heads) return;
+    h = 0;
+    for (++b; b < p.batch; ++b) {
+      load();
+      if (r.n > 0) return;
+    }
+    left = 0;
+  }
+  __device__ bool next(Piece& s) {
+    while (left > 0) {
+      const int units = item_units(p, r, qt, tpt);
+      if (tile >= units) {
+        advance();
+        continue;
+      }
+      s.b = b;
+      s.h = h;
+      s.qt = qt;
+      s.r = r;
+      s.units = units;
+      s.a = tile;
+      s.e = (int)min((long long)units, tile + left);
+      left -= s.e - s.a;
+      const int tok = qt * 2 * tpt, n = min(2 * tpt, r.n - tok);
+      s.end[0] = max(s.a, min(s.e, max(1, div_up(visible(p, r, tok + min(n, tpt) - 1), kKeys))));
+      s.end[1] = n > tpt ? s.e : s.a;
+      s.edge = visible(p, r, tok) / kKeys;
+      if (left > 0) advance();
+      return true;
+    }
+    return false;
+  }
+};
+
+// ------------------------------------------------------- partial results ----
+// Block c leaves at most two: slot 0 for an item that an earlier block began,
+// slot 1 for one that a later block goes on with.
+struct Piece2Join {
+  int head;      // 0 empty range, 1 slot 0 goes on in a later block, 2 slot 0 ends the item, 3 begins with an item
+  int tail;      // slot 1 holds the beginning of an item
+  int first, n;  // that item's first row (absolute) and its rows' tokens
+  int h;
+  int pad[3];
+};
+template <int D> struct Slot {
+  float o[D / 4][2 * kRows][4];          // column blocks of four, so that a warp's rows are adjacent
+  float2 ml[2 * kRows];                  // maximum, sum
+};
+
+template <int D> struct Cfg {
+  static constexpr int HALVES = D / 64;
+  static constexpr int HALF = kKeys * 128;                   // 128 rows x 64 elements
+  static constexpr int TILE = HALVES * HALF;
+  static constexpr int ST = D == 128 ? 2 : 4;                // K and V steps in flight
+  static constexpr int K0 = 2 * TILE, V0 = K0 + ST * TILE, BARS = V0 + ST * TILE;
+  enum : int { B_QF = 0, B_QE = 1, B_SF = 2, B_PF = 4, B_OF = 6, B_KF = 8, B_KE = B_KF + ST, B_VF = B_KE + ST,
+               B_VE = B_VF + ST, B_VG = B_VE + ST, B_END = B_VG + ST, B_N };
+  static constexpr int BYTES = BARS + 1024 /* barriers, flags */ + 1024 /* alignment */;
+};
+
+struct Maps {
+  CUtensorMap q, k, v;
+  int tpt;                               // tokens of a tile: 128 / group
+  int box;                               // keys of one K or V copy
+  void* partial;
+  Piece2Join* join;
+};
+
+// Byte of element (row, col) of a 128-byte-swizzled tile.
+__device__ __forceinline__ uint32_t swizzled(int row, int col, int half_bytes) {
+  return (col >> 6) * half_bytes + row * 128 + ((((col & 63) * 2) >> 4 ^ (row & 7)) << 4) + ((col & 7) * 2);
+}
+
+// O (+)= P V for one row on the CUDA cores: the step's V holds a NaN or an
+// infinity that this row may not see, and a matrix product would spread it.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) row_kernel(const Params p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int t = (int)(w / p.heads), h = (int)(w - (int64_t)t * p.heads);
-  if (t >= p.tokens) return;
-  int a = 0, e = p.batch;
-  while (e - a > 1) {
-    const int mid = (a + e) >> 1;
-    if (p.starts[mid] <= t) a = mid; else e = mid;
-  }
-  const Request r = request(p, a);
-  if (t < r.first || t >= r.first + r.n) return;
-  const int limit = p.causal ? max(0, r.keys - r.n + (t - r.first) + 1) : r.keys;
-  const int hk = h / p.group;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < E; ++i) {
-    q[i] = to_f32(static_cast<const T*>(p.q)[t * p.q_ts + h * p.q_hs + lane * E + i]) * p.scale * 1.4426950408889634f;
-    o[i] = 0.f;
-  }
-  for (int j = 0; j < limit; ++j) {
-    int64_t kb, vb;
-    bool in = true;
-    if (p.table) {
-      const int block = p.table[a * p.table_stride + j / p.page];
-      in = block >= 0 && block < p.num_blocks;
-      kb = block * p.k_bs + (j % p.page) * p.k_ts;
-      vb = block * p.v_bs + (j % p.page) * p.v_ts;
+__device__ __noinline__ void careful_pv(uint32_t tP, uint32_t tO, const unsigned char* v, bool first, int lim) {
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    uint32_t o[32];
+    if (first) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = 0u;
     } else {
-      kb = (r.first + j) * p.k_ts;
-      vb = (r.first + j) * p.v_ts;
+      tmem_ld32(tO + c, o);
+      tmem_wait_ld();
     }
-    float s = 0.f, vv[E];
-    for (int i = 0; i < E; ++i) {
-      s = fmaf(q[i], in ? to_f32(static_cast<const T*>(p.k)[kb + hk * p.k_hs + lane * E + i]) : 0.f, s);
-      vv[i] = in ? to_f32(static_cast<const T*>(p.v)[vb + hk * p.v_hs + lane * E + i]) : 0.f;
+#pragma unroll 1
+    for (int k = 0; k < kKeys; k += 16) {
+      uint32_t pw[8];
+      tmem_ld8(tP + k / 2, pw);
+      tmem_wait_ld();
+#pragma unroll 1
+      for (int kk = 0; kk < 16; ++kk) {
+        uint32_t word = pw[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) word = (kk >> 1) == i ? pw[i] : word;
+        const float2 pp = unpack2<T>(word);
+        const float pj = kk & 1 ? pp.y : pp.x;
+        const bool seen = k + kk < lim;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4*>(v + swizzled(k + kk, c + 8 * i, Cfg<D>::HALF));
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 f = unpack2<T>(w[q]);
+            const int at = 8 * i + 2 * q;
+            if (seen) {
+              o[at] = __float_as_uint(fmaf(pj, f.x, __uint_as_float(o[at])));
+              o[at + 1] = __float_as_uint(fmaf(pj, f.y, __uint_as_float(o[at + 1])));
+            }
+          }
+        }
+      }
     }
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s);
-    const float al = exp2f(m - mn), pr = exp2f(s - mn);
-    m = mn;
-    l = l * al + pr;
-    for (int i = 0; i < E; ++i) o[i] = o[i] * al + pr * vv[i];
+    tmem_st32(tO + c, o);
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  for (int i = 0; i < E; ++i)
-    static_cast<T*>(p.out)[t * p.o_ts + h * p.o_hs + lane * E + i] = from_f32<T>(o[i] * inv);
+  tmem_wait_st();
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ Maps maps, const Params p) {
+  using C = Cfg<D>;
+  constexpr int ST = C::ST;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ ScanSpace scan;
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::B_N);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* vflag = abort_flag + 1;  // [ST][2]: NaN or infinity found by each guard warp
+  const uint32_t bar0 = smem_u32(bars);
+#define BAR(i) (bar0 + 8u * (uint32_t)(i))
+#define WAIT(i, parity, code) mbar_wait(BAR(i), (parity), abort_flag, &g_fault, (code))
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  launch_dependents();
+  if (threadIdx.x == 0) {
+    mbar_init(BAR(C::B_QF), 1);
+    mbar_init(BAR(C::B_QE), 1);
+    mbar_init(BAR(C::B_END), 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(BAR(C::B_SF + t), 1);
+      mbar_init(BAR(C::B_PF + t), 4);    // one arrival per softmax warp
+      mbar_init(BAR(C::B_OF + t), 1);
+    }
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(BAR(C::B_KF + s), 1);
+      mbar_init(BAR(C::B_KE + s), 1);
+      mbar_init(BAR(C::B_VF + s), 1);
+      mbar_init(BAR(C::B_VE + s), 1);
+      mbar_init(BAR(C::B_VG + s), 2);    // one arrival per guard warp
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 9) tmem_alloc_512(smem_u32(tmem_slot));
+  Range range;
+  find_range(p, maps.tpt, blockIdx.x, gridDim.x, scan, range);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t sq = smem_u32(smem), sk = sq + C::K0, sv = sq + C::V0;
+  const int tpt = maps.tpt;
+  Walk walk(p, tpt, range);
+  Piece s;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------- producer --
+    const int boxes = kKeys / maps.box;
+    const int bx = lane % boxes, half = lane / boxes;         // this lane's copy of a step
+    const bool mine = lane < boxes * C::HALVES;
+    const uint32_t dst = half * C::HALF + bx * maps.box * 128;
+    uint32_t it = 0, pieces = 0;
+    bool ok = true;
+    if (lane == 0) {
+      tma_prefetch_map(&maps.q);
+      tma_prefetch_map(&maps.k);
+      tma_prefetch_map(&maps.v);
+    }
+    uint32_t v_issued = 0;
+    while (ok && walk.next(s)) {
+      for (int j = s.a; j < s.e && ok; ++j, ++it) {
+        // coordinates of this lane's keys; a block outside the cache reads as zeros
+        int z, w = 0;
+        const int key = j * kKeys + bx * maps.box;
+        if (p.table) {
+          const int pg = key / p.page;
+          z = key - pg * p.page;
+          int block = -1;
+          if (mine && key < s.r.keys) block = p.table[(int64_t)s.b * p.table_stride + pg];
+          w = block >= 0 && block < p.num_blocks ? block : -1;
+        } else {
+          z = s.r.first + key;
+        }
+        const int st = it % ST;
+        const uint32_t ph = (it / ST) & 1;
+        ok = WAIT(C::B_KE + st, ph ^ 1, 1);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) mbar_expect_tx(BAR(C::B_KF + st), C::TILE);
+        __syncwarp();
+        if (mine) tma_load_4d(sk + st * C::TILE + dst, &maps.k, half * 64, s.h, z, w, BAR(C::B_KF + st));
+        if (j == s.a) {
+          ok = WAIT(C::B_QE, (pieces & 1) ^ 1, 2);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ++it;
+            break;
+          }
+          const int tok = s.qt * 2 * tpt, tiles = s.r.n - tok > tpt ? 2 : 1;
+          if (lane == 0) mbar_expect_tx(BAR(C::B_QF), tiles * D * 2 * p.group * tpt);
+          __syncwarp();
+          if (lane < tiles * C::HALVES) {
+            const int t = lane / C::HALVES, hf = lane % C::HALVES;
+            tma_load_4d(sq + t * C::TILE + hf * C::HALF, &maps.q, hf * 64, 0, s.h, s.r.first + tok + t * tpt,
+                        BAR(C::B_QF));
+          }
+          ++pieces;
+        }
+        ok = WAIT(C::B_VE + st, ph ^ 1, 3);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ++it;
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(BAR(C::B_VF + st), C::TILE);
+        __syncwarp();
+        if (mine) tma_load_4d(sv + st * C::TILE + dst, &maps.v, half * 64, s.h, z, w, BAR(C::B_VF + st));
+        v_issued = it + 1;
+      }
+      if (!__all_sync(0xffffffffu, ok)) break;
+    }
+    // Every copy issued lands before the block leaves.
+    if (lane == 0) {
+      for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i) mbar_drain(BAR(C::B_KF + i % ST), (i / ST) & 1);
+      for (uint32_t i = v_issued > ST ? v_issued - ST : 0; i < v_issued; ++i)
+        mbar_drain(BAR(C::B_VF + i % ST), (i / ST) & 1);
+      if (pieces) mbar_drain(BAR(C::B_QF), (pieces - 1) & 1);
+    }
+  } else if (warp == 9) {
+    // ----------------------------------------------------------- MMA issuer --
+    if (lane == 0) {
+      constexpr uint32_t ID_QK = instr_desc<T>(kRows, kKeys, false);
+      constexpr uint32_t ID_PV = instr_desc<T>(kRows, D, true);
+      auto qk = [&](int t, int st) {     // S_t = Q_t K^T
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * C::HALF + (kk & 3) * 32;
+          mma_ss(tmem + 256 + 128 * t, smem_desc(sq + t * C::TILE + off, 16), smem_desc(sk + st * C::TILE + off, 16),
+                 ID_QK, kk != 0);
+        }
+        mma_commit(BAR(C::B_SF + t));
+      };
+      auto pv = [&](int t, int st, bool acc) {   // O_t (+)= P_t V
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_ts(tmem + 128 * t, tmem + 256 + 128 * t + kk * 8, smem_desc(sv + st * C::TILE + kk * 2048, C::HALF),
+                 ID_PV, (acc || kk != 0) ? 1u : 0u);
+      };
+      uint32_t it = 0, pieces = 0, seen[2] = {0, 0};
+      bool more = walk.next(s), ok = true;
+      int j = s.a;
+      if (more) {
+        ok = WAIT(C::B_QF, 0, 4) && WAIT(C::B_KF, 0, 5);
+        if (ok) {
+          fence_after();
+          for (int t = 0; t < 2; ++t)
+            if (j < s.end[t]) qk(t, 0);
+          mma_commit(BAR(C::B_KE));
+          if (j + 1 == s.e) mma_commit(BAR(C::B_QE));
+        }
+      }
+      while (more && ok) {
+        Piece ns = s;
+        int nj = j + 1;
+        const bool turn = nj == s.e;     // the next step begins another piece
+        if (turn) {
+          more = walk.next(ns);
+          nj = ns.a;
+          ++pieces;
+        }
+        const int st = it % ST, nst = (it + 1) % ST;
+        if (!WAIT(C::B_VG + st, (it / ST) & 1, 6)) break;
+        const bool careful = vflag[2 * st] | vflag[2 * st + 1];
+        bool waited = false;
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j < s.end[t]) {
+            ok = WAIT(C::B_PF + t, seen[t] & 1, 7 + t);
+            if (!ok) break;
+            ++seen[t];
+            fence_after();
+            if (!careful) pv(t, st, j > s.a);
+            if (j + 1 == s.end[t]) mma_commit(BAR(C::B_OF + t));
+          }
+          if (t == 1) mma_commit(BAR(C::B_VE + st));
+          if (more && nj < ns.end[t]) {
+            if (!waited) {
+              ok = (!turn || WAIT(C::B_QF, pieces & 1, 9)) && WAIT(C::B_KF + nst, ((it + 1) / ST) & 1, 10);
+              if (!ok) break;
+              fence_after();
+              waited = true;
+            }
+            qk(t, nst);
+          }
+        }
+        if (!ok) break;
+        if (more) {
+          mma_commit(BAR(C::B_KE + nst));
+          if (nj + 1 == ns.e) mma_commit(BAR(C::B_QE));
+        }
+        s = ns;
+        j = nj;
+        ++it;
+      }
+      // Every MMA issued completes before tensor memory is freed.
+      mma_commit(BAR(C::B_END));
+      mbar_drain(BAR(C::B_END), 0);
+    }
+  } else if (warp >= 10) {
+    // --------------------------------------------------------- guards of V --
+    const int g = warp - 10;
+    uint32_t it = 0;
+    bool ok = true;
+    Piece2Join jn{range.units > 0 ? 3 : 0, 0, 0, 0, 0, {0, 0, 0}};
+    while (ok && walk.next(s)) {
+      const int tok = s.qt * 2 * tpt;
+      if (s.a > 0) jn.head = s.e == s.units ? 2 : 1;          // only the first piece begins inside an item
+      if (s.a == 0 && s.e < s.units) {                        // only the last one ends inside one
+        jn.tail = 1;
+        jn.first = s.r.first + tok;
+        jn.n = min(2 * tpt, s.r.n - tok);
+        jn.h = s.h;
+      }
+      const int some = visible(p, s.r, tok);                                  // seen by every row
+      const int most = visible(p, s.r, min(s.r.n, tok + 2 * tpt) - 1);        // seen by any
+      for (int j = s.a; j < s.e; ++j, ++it) {
+        const int st = it % ST;
+        ok = __all_sync(0xffffffffu, WAIT(C::B_VF + st, (it / ST) & 1, 11));
+        if (!ok) break;
+        int bad = 0;
+        if (j >= s.edge) {
+          unsigned char* v = smem + C::V0 + st * C::TILE;
+          const int lo = max(0, some - j * kKeys), hi = min(kKeys, max(0, most - j * kKeys));
+          constexpr int CH = D / 8;      // 16-byte vectors of a row
+          for (int i = lo * CH + g * 32 + lane; i < kKeys * CH; i += 64) {
+            const int row = i / CH, col = (i % CH) * 8;
+            uint4* x = reinterpret_cast<uint4*>(v + swizzled(row, col, C::HALF));
+            if (row >= hi) {
+              *x = make_uint4(0, 0, 0, 0);
+            } else {
+              constexpr uint32_t E = Bits16<T>::kInf * 0x10001u, EL = Bits16<T>::kInf, EH = EL << 16;
+              const uint4 y = *x;
+              const uint32_t w[4] = {y.x & E, y.y & E, y.z & E, y.w & E};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) bad |= (w[q] & EL) == EL || (w[q] & EH) == EH;
+            }
+          }
+          fence_async_smem();
+        }
+        bad = __any_sync(0xffffffffu, bad);
+        if (lane == 0) {
+          vflag[2 * st + g] = bad;
+          mbar_arrive(BAR(C::B_VG + st));
+        }
+      }
+    }
+    // what join_kernel needs to know of this block's range
+    if (g == 0 && lane == 0 && maps.join) {
+      if (!ok) jn = Piece2Join{0, 0, 0, 0, 0, {0, 0, 0}};
+      maps.join[blockIdx.x] = jn;
+    }
+  } else {
+    // -------------------------------------------------------------- softmax --
+    const int t = warp >> 2;                       // tile of this warpgroup
+    const int row = (warp & 3) * 32 + lane;        // TMEM lane
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + 256 + t * 128 + lane_off;
+    const uint32_t tO = tmem + t * 128 + lane_off;
+    const float c = p.scale_log2;
+    const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+    uint32_t it = 0, tiles = 0, outs = 0;
+    bool ok = true;
+    while (ok && walk.next(s)) {
+      const int i_tok = s.qt * 2 * tpt + t * tpt + row_tok;
+      const bool valid = row_tok < tpt && i_tok < s.r.n;
+      const int limit = visible(p, s.r, min(i_tok, s.r.n - 1));
+      float m = kNoMax;                            // running max of s * c (may lag the true one by less than 8)
+      float l = 0.f;                               // running sum
+      for (int j = s.a; j < s.e; ++j, ++it) {
+        if (j >= s.end[t]) continue;
+        ok = __all_sync(0xffffffffu, WAIT(C::B_SF + t, tiles & 1, 12));
+        if (!ok) break;
+        ++tiles;
+        fence_after();
+        float x[128];
+        uint32_t* xu = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, xu + q * 32);
+        tmem_wait_ld();
+        if (p.negate) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) x[i] = -x[i];
+        }
+        const bool edge = j >= s.edge;
+        const int lim = limit - j * kKeys;
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i >= lim) x[i] = -INFINITY;
+        }
+        float mq[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int i = 4; i < 124; i += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mq[q] = max3f(mq[q], x[i + 2 * q], x[i + 2 * q + 1]);
+        mq[0] = max3f(mq[0], x[124], x[125]);
+        mq[1] = max3f(mq[1], x[126], x[127]);
+        const float mt = max3f(mq[0], mq[1], fmaxf(mq[2], mq[3])) * c;
+        const bool need = mt > m + 8.f;
+        const bool any_need = __any_sync(0xffffffffu, need);
+        const float m_new = need ? mt : m;
+        const float alpha = ex2(m - m_new);        // 1 where the max is kept; 0 at the first visible key
+        m = m_new;
+        const float2 c2 = make_float2(c, c), mn2 = make_float2(-m, -m);
+        float2 ra[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 32 * ch; i < 32 * ch + 32; i += 2) {
+            float2 e = fma2(make_float2(x[i], x[i + 1]), c2, mn2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            pk[(i - 32 * ch) >> 1] = pack2<T>(e.x, e.y);
+            ra[(i >> 1) & 3] = add2(ra[(i >> 1) & 3], e);
+          }
+          tmem_st16(tS + 16 * ch, pk);
+        }
+        const float2 r01 = add2(ra[0], ra[1]), r23 = add2(ra[2], ra[3]);
+        l = __fmaf_rn(l, alpha, (r01.x + r01.y) + (r23.x + r23.y));
+        // O_t *= alpha (PV_t of the step before has completed: it was issued
+        // before the QK_t that released this S).
+        if (any_need && j > s.a) {
+#pragma unroll 1
+          for (int q = 0; q < D; q += 32) {
+            uint32_t o[32];
+            tmem_ld32(tO + q, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(tO + q, o);
+          }
+        }
+        tmem_wait_st();
+        if (edge) {
+          const int st = it % ST;
+          ok = __all_sync(0xffffffffu, WAIT(C::B_VG + st, (it / ST) & 1, 13));
+          if (!ok) break;
+          if (vflag[2 * st] | vflag[2 * st + 1])
+            careful_pv<T, D>(tS, tO, smem + C::V0 + st * C::TILE, j == s.a, lim);
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(C::B_PF + t));
+      }
+      if (!ok) break;
+      // ---- epilogue ----
+      const bool has = s.end[t] > s.a;
+      if (has) {
+        ok = __all_sync(0xffffffffu, WAIT(C::B_OF + t, outs & 1, 14));
+        if (!ok) break;
+        ++outs;
+        fence_after();
+      }
+      const bool whole = s.a == 0 && s.e == s.units;
+      if (whole) {
+        if (!has) continue;
+        // a row that sees no key has l = 0 and an O that was never scaled: zero
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T* orow = static_cast<T*>(p.out) + (int64_t)(s.r.first + i_tok) * p.o_ts +
+                  (int64_t)(s.h * p.group + row_head) * p.o_hs;
+#pragma unroll 1
+        for (int q = 0; q < D; q += 32) {
+          uint32_t o[32];
+          tmem_ld32(tO + q, o);
+          tmem_wait_ld();
+          if (valid) {
+            uint4* dst = reinterpret_cast<uint4*>(orow + q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float lo = __uint_as_float(o[8 * i + 2 * k]), hi = __uint_as_float(o[8 * i + 2 * k + 1]);
+                w[k] = l == 0.f ? 0u : pack2<T>(lo * inv, hi * inv);
+              }
+              dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      } else {
+        Slot<D>& slot = static_cast<Slot<D>*>(maps.partial)[2 * blockIdx.x + (s.a == 0 ? 1 : 0)];
+        const int r2 = t * kRows + row;
+        slot.ml[r2] = make_float2(m, l);
+        if (has) {
+#pragma unroll 1
+          for (int q = 0; q < D; q += 32) {
+            uint32_t o[32];
+            tmem_ld32(tO + q, o);
+            tmem_wait_ld();
+            if (valid) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<uint4*>(slot.o[q / 4 + i][r2]) =
+                    make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+          }
+        }
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 9) tmem_free_512(tmem);
+#undef BAR
+#undef WAIT
+}
+
+// Adds up the partial results of the items that cuts divide.  Block (c, y):
+// the item whose first piece is block c's last; a warp takes 32 rows and 8
+// columns of it (y enumerates them), each lane one row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join_kernel(const Params p, const Slot<D>* slots, const Piece2Join* join, int tpt,
+                                                   int blocks) {
+  __shared__ int heads[kMaxBlocks];
+  wait_for_primary();
+  const Piece2Join me = join[blockIdx.x];
+  if (!me.tail) return;
+  for (int i = threadIdx.x; i < blocks; i += blockDim.x) heads[i] = join[i].head;
+  __syncthreads();
+  const int w = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int col = (w % (D / 8)) * 8, r2 = (w / (D / 8)) * 32 + lane;
+  const int t = r2 / kRows, row = r2 % kRows;
+  const int tok_in_tile = row / p.group, tok = t * tpt + tok_in_tile;
+  if (tok_in_tile >= tpt || tok >= me.n) return;
+  float m = kNoMax, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  int c = blockIdx.x, slot = 2 * c + 1;
+  bool last = false;
+  while (true) {
+    const Slot<D>& s = slots[slot];
+    const float2 ml = s.ml[r2];
+    const float4 x = *reinterpret_cast<const float4*>(s.o[col / 4][r2]);
+    const float4 y = *reinterpret_cast<const float4*>(s.o[col / 4 + 1][r2]);
+    if (ml.y != 0.f) {                   // rows without a visible key there have no O either
+      const float mn = fmaxf(m, ml.x), a = ex2(m - mn), b = ex2(ml.x - mn);
+      m = mn;
+      l = l * a + ml.y * b;
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = o[i] * a + v[i] * b;
+    }
+    if (last) break;
+    int head = 0;
+    while (++c < blocks && (head = heads[c]) == 0) {
+    }
+    if (c >= blocks || head == 3) break;
+    slot = 2 * c;
+    last = head == 2;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint32_t out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = pack2<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
+  T* dst = static_cast<T*>(p.out) + (int64_t)(me.first + tok) * p.o_ts + (int64_t)(me.h * p.group + row % p.group) * p.o_hs + col;
+  *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+// ------------------------------------------------------------------- host --
+static int64_t join_bytes(int blocks) { return (int64_t)blocks * (int64_t)sizeof(Piece2Join); }
+static int64_t slot_bytes(int head_dim) {
+  return head_dim == 64 ? (int64_t)sizeof(Slot<64>) : (int64_t)sizeof(Slot<128>);
+}
+static int tile_blocks() { return sm_count() < kMaxBlocks ? sm_count() : kMaxBlocks; }
+static int64_t workspace_bytes_for(int head_dim) {
+  const int n = tile_blocks();
+  return join_bytes(n) + 2 * (int64_t)n * slot_bytes(head_dim);
 }
 
 static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
-                 int64_t head_dim, int dtype) {
+                 int64_t head_dim, float scale, int dtype) {
   JO_REQUIRE(dtype == JO_DTYPE_BF16 || dtype == JO_DTYPE_F16, JO_ERR_DTYPE, "%s: only bf16 and fp16 are supported", what);
   JO_REQUIRE(head_dim == 64 || head_dim == 128, JO_ERR_INVALID, "%s: head_dim must be 64 or 128 (got %lld)", what,
              (long long)head_dim);
   JO_REQUIRE(tokens >= 0 && batch >= 0 && heads >= 0 && kv_heads >= 0 && tokens < (1LL << 30) && batch < (1LL << 30) &&
                  heads < 65536,
              JO_ERR_INVALID, "%s: invalid shape", what);
-  JO_REQUIRE(heads == 0 || (kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 128), JO_ERR_INVALID,
+  JO_REQUIRE(heads == 0 || (kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= kRows), JO_ERR_INVALID,
              "%s: heads (%lld) must be a multiple of kv_heads (%lld), at most 128 times it", what, (long long)heads,
              (long long)kv_heads);
   const int64_t s[10] = {p.q_ts, p.q_hs, p.k_bs, p.k_ts, p.k_hs, p.v_bs, p.v_ts, p.v_hs, p.o_ts, p.o_hs};
@@ -107,29 +812,92 @@ static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int
     JO_REQUIRE(s[i] >= 0 && s[i] % 8 == 0, JO_ERR_ALIGN, "%s: strides must be non-negative multiples of 8 elements", what);
   JO_REQUIRE(aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.out), JO_ERR_ALIGN,
              "%s: tensors must be 16-byte aligned", what);
+  JO_REQUIRE(isfinite(scale), JO_ERR_INVALID, "%s: scale must be finite", what);
   p.tokens = (int)tokens;
   p.batch = (int)batch;
   p.heads = (int)heads;
+  p.kv_heads = (int)kv_heads;
   p.group = kv_heads > 0 ? (int)(heads / kv_heads) : 1;
   p.head_dim = (int)head_dim;
+  // a masked score is -infinity and must stay so after the scaling, at scale 0 too
+  p.scale_log2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);
+  p.negate = scale < 0.f;
   return JO_OK;
 }
 
-static int launch(const char* what, const Params& p, int dtype, void* stream) {
+template <typename T, int D>
+static int launch_tiles(const char* what, const Params& p, void* workspace, cudaStream_t stream) {
+  constexpr bool bf16 = IsBf16<T>::v;
+  Maps maps;
+  maps.tpt = kRows / p.group;
+  const int blocks = tile_blocks();
+  const int64_t qd[4] = {D, p.group, p.kv_heads, p.tokens}, qs[3] = {p.q_hs, p.q_hs * p.group, p.q_ts};
+  const int qb[4] = {64, p.group, 1, maps.tpt};
+  bool ok = make_map_4d(&maps.q, bf16, p.q, qd, qs, qb);
+  if (p.table) {
+    maps.box = p.page & -p.page;                     // the largest power of two that divides the page
+    if (maps.box > kKeys) maps.box = kKeys;
+    const int kb[4] = {64, 1, maps.box, 1};
+    // an empty cache: every block is outside it, the address is never read
+    const int64_t d[4] = {D, p.kv_heads, p.page, p.num_blocks > 0 ? p.num_blocks : 1};
+    const int64_t ks[3] = {p.k_hs, p.k_ts, p.k_bs}, vs[3] = {p.v_hs, p.v_ts, p.v_bs};
+    ok = ok && make_map_4d(&maps.k, bf16, p.num_blocks > 0 ? p.k : p.q, d, ks, kb) &&
+         make_map_4d(&maps.v, bf16, p.num_blocks > 0 ? p.v : p.q, d, vs, kb);
+  } else {
+    maps.box = kKeys;
+    const int kb[4] = {64, 1, kKeys, 1};
+    const int64_t d[4] = {D, p.kv_heads, p.tokens, 1};
+    const int64_t ks[3] = {p.k_hs, p.k_ts, 0}, vs[3] = {p.v_hs, p.v_ts, 0};
+    ok = ok && make_map_4d(&maps.k, bf16, p.k, d, ks, kb) && make_map_4d(&maps.v, bf16, p.v, d, vs, kb);
+  }
+  if (!ok) {
+    set_error("%s: cuTensorMapEncodeTiled failed", what);
+    return JO_ERR_CUDA;
+  }
+  // No item has a cut inside when none is long enough to have one away from its edges.
+  const int64_t most_keys = p.table ? (int64_t)p.width * p.page : p.tokens;
+  const bool split = most_keys > (2 * kMinPiece - 1) * kKeys;
+  maps.join = split ? static_cast<Piece2Join*>(workspace) : nullptr;
+  maps.partial = static_cast<char*>(workspace) + join_bytes(blocks);
+  static bool attr[kMaxDevices] = {};
+  const int dev = device_slot();
+  if (!attr[dev]) {
+    if (cudaFuncSetAttribute(tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::BYTES) != cudaSuccess)
+      return check_launch(what);
+    attr[dev] = true;
+  }
+  tile_kernel<T, D><<<blocks, kThreads, Cfg<D>::BYTES, stream>>>(maps, p);
+  if (split) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks, 2 * kRows / 32 * (D / 8) / 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p, static_cast<const Slot<D>*>(maps.partial),
+                       static_cast<const Piece2Join*>(maps.join), maps.tpt, blocks);
+  }
+  return check_launch(what);
+}
+
+static int launch(const char* what, const Params& p, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (p.tokens == 0 || p.batch == 0 || p.heads == 0) return JO_OK;
   JO_REQUIRE(p.q && p.out && p.starts, JO_ERR_INVALID, "%s: null tensor pointer", what);
   int st = require_sm100();
   if (st != JO_OK) return st;
-  const unsigned grid = (unsigned)(((int64_t)p.tokens * p.heads + 3) / 4);
+  const int64_t need = workspace_bytes_for(p.head_dim);
+  JO_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, JO_ERR_INVALID,
+             "%s: a 16-byte aligned workspace of %lld bytes is needed (got %lld)", what, (long long)need,
+             (long long)workspace_bytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == JO_DTYPE_BF16) {
-    if (p.head_dim == 64) row_kernel<__nv_bfloat16, 64><<<grid, 128, 0, s>>>(p);
-    else row_kernel<__nv_bfloat16, 128><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (p.head_dim == 64) row_kernel<__half, 64><<<grid, 128, 0, s>>>(p);
-    else row_kernel<__half, 128><<<grid, 128, 0, s>>>(p);
-  }
-  return check_launch(what);
+  if (dtype == JO_DTYPE_BF16)
+    return p.head_dim == 64 ? launch_tiles<__nv_bfloat16, 64>(what, p, workspace, s)
+                            : launch_tiles<__nv_bfloat16, 128>(what, p, workspace, s);
+  return p.head_dim == 64 ? launch_tiles<__half, 64>(what, p, workspace, s)
+                          : launch_tiles<__half, 128>(what, p, workspace, s);
 }
 
 }  // namespace vattn
@@ -158,12 +926,12 @@ int jo_paged_attention(const void* q, const void* key_cache, const void* value_c
   p.page = (int)page_size;
   p.width = (int)table_width;
   p.causal = causal != 0;
-  p.scale = scale;
-  int st = vattn::check(what, p, tokens, batch, heads, kv_heads, head_dim, dtype);
+  int st = vattn::check(what, p, tokens, batch, heads, kv_heads, head_dim, scale, dtype);
   if (st != JO_OK) return st;
   JO_REQUIRE(tokens == 0 || batch == 0 || (kv_lens && block_tables && (num_blocks == 0 || (key_cache && value_cache))),
              JO_ERR_INVALID, "%s: null tensor pointer", what);
-  return vattn::launch(what, p, dtype, stream);
+  (void)max_query_len;
+  return vattn::launch(what, p, dtype, workspace, workspace_bytes, stream);
 }
 
 int jo_prompt_attention(const void* q, const void* k, const void* v, const int32_t* seq_starts, void* out,
@@ -180,18 +948,35 @@ int jo_prompt_attention(const void* q, const void* k, const void* v, const int32
   p.page = 1;
   p.width = 0;
   p.causal = causal != 0;
-  p.scale = scale;
-  int st = vattn::check(what, p, tokens, batch, heads, kv_heads, head_dim, dtype);
+  int st = vattn::check(what, p, tokens, batch, heads, kv_heads, head_dim, scale, dtype);
   if (st != JO_OK) return st;
   JO_REQUIRE(tokens == 0 || batch == 0 || (k && v), JO_ERR_INVALID, "%s: null tensor pointer", what);
-  return vattn::launch(what, p, dtype, stream);
+  return vattn::launch(what, p, dtype, workspace, workspace_bytes, stream);
 }
 
 int jo_varlen_attention_workspace(int64_t tokens, int64_t heads, int64_t head_dim, int64_t* bytes) {
+  using namespace jo;
   JO_REQUIRE(bytes, JO_ERR_INVALID, "varlen_attention_workspace: null pointer");
-  (void)tokens, (void)heads, (void)head_dim;
-  *bytes = 0;
+  JO_REQUIRE(head_dim == 64 || head_dim == 128, JO_ERR_INVALID,
+             "varlen_attention_workspace: head_dim must be 64 or 128 (got %lld)", (long long)head_dim);
+  (void)tokens, (void)heads;
+  *bytes = vattn::workspace_bytes_for((int)head_dim);
   return JO_OK;
+}
+
+// Fault code of the kernels' bounded waits (0 = none); reset != 0 clears it.
+// One sticky value per device, shared by every launch.  Synchronous.
+int jo_varlen_attention_last_fault(int reset) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, jo::vattn::g_fault, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return JO_ERR_CUDA;
+  }
+  if (reset) {
+    int z = 0;
+    cudaMemcpyToSymbol(jo::vattn::g_fault, &z, sizeof(int));
+  }
+  return v;
 }
 
 }  // extern "C"

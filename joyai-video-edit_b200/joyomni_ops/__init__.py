@@ -427,7 +427,8 @@ def check_gemm_fault(device=None) -> None:
     with torch.cuda.device(dev):
         torch.cuda.synchronize(dev)
         codes = {"fp8_scaled_mm": _L.jo_gemm_last_fault(1) if has_fp8() else 0,
-                 "attention": _L.jo_attention_last_fault(1)}
+                 "attention": _L.jo_attention_last_fault(1),
+                 "paged_attention / prompt_attention": _L.jo_varlen_attention_last_fault(1)}
     for name, code in codes.items():
         if code < 0:
             _check(code)
