@@ -262,14 +262,13 @@ int jo_paged_layout(const int32_t* cached_lens, const int32_t* new_lens, int32_t
 /*
  * Stores rows of key and value [tokens, kv_heads, head_dim] into their slots of
  * the caches; rows whose slot is negative or past the cache are left out.
- * k_strides, v_strides: token and head strides; kc_strides, vc_strides: block,
- * token and head strides (elements, multiples of 8, rows of head_dim elements
- * dense).  head_dim % 8 == 0; dtype JO_DTYPE_BF16/F16; 16-byte aligned tensors.
+ * row_strides: token and head strides of key, then of value; cache_strides:
+ * block, token and head strides of key_cache, then of value_cache (elements,
+ * multiples of 8, rows of head_dim elements dense).  head_dim % 8 == 0; dtype JO_DTYPE_BF16/F16; 16-byte aligned tensors.
  */
 int jo_paged_kv_write(const void* key, const void* value, void* key_cache, void* value_cache, const int64_t* slots,
                       int64_t tokens, int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t page_size,
-                      const int64_t* k_strides, const int64_t* v_strides, const int64_t* kc_strides,
-                      const int64_t* vc_strides, int dtype, void* stream);
+                      const int64_t* row_strides, const int64_t* cache_strides, int dtype, void* stream);
 
 /*
  * Attention of new tokens (one or a chunk a request) over a paged cache:
@@ -284,29 +283,30 @@ int jo_paged_kv_write(const void* key, const void* value, void* key_cache, void*
  * max_query_len: the largest number of new tokens of a request, as far as the
  * host knows it (it only chooses the kernels; any value gives the result).
  * head_dim 64 or 128; dtype JO_DTYPE_BF16/F16; page_size % 16 == 0;
- * heads / kv_heads <= 128.  Strides (elements, multiples of 8): q, out: token
- * and head; caches: block, token and head.  workspace: at least
+ * heads / kv_heads <= 128.  row_strides: token and head strides of q, then of
+ * out; cache_strides: block, token and head strides of key_cache, then of
+ * value_cache (elements, multiples of 8).  workspace: at least
  * jo_varlen_attention_workspace bytes, 16-byte aligned, used by one call at a
  * time.
  */
 int jo_paged_attention(const void* q, const void* key_cache, const void* value_cache, const int32_t* block_tables,
                        const int32_t* query_starts, const int32_t* kv_lens, void* out, int64_t tokens, int64_t batch,
                        int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t page_size,
-                       int64_t table_width, int64_t table_stride, const int64_t* q_strides, const int64_t* kc_strides,
-                       const int64_t* vc_strides, const int64_t* o_strides, int causal, float scale,
-                       int64_t max_query_len, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+                       int64_t table_width, int64_t table_stride, const int64_t* row_strides,
+                       const int64_t* cache_strides, int causal, float scale, int64_t max_query_len, int dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Attention of whole packed prompts: request b is rows seq_starts[b] ..
  * seq_starts[b + 1] of q [tokens, heads, head_dim] and of k, v [tokens,
  * kv_heads, head_dim]; row i sees keys 0 .. i (causal != 0) or all of its own
- * request.  Everything else as jo_paged_attention; strides: token and head.
+ * request.  Everything else as jo_paged_attention; kv_strides: token and head
+ * strides of k, then of v.
  */
 int jo_prompt_attention(const void* q, const void* k, const void* v, const int32_t* seq_starts, void* out,
                         int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                        const int64_t* o_strides, int causal, float scale, int dtype, void* workspace,
-                        int64_t workspace_bytes, void* stream);
+                        const int64_t* row_strides, const int64_t* kv_strides, int causal, float scale, int dtype,
+                        void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Bytes of workspace that the two calls above need for these sizes (the
  * partial results of work that is split along the keys). */

@@ -211,8 +211,7 @@ int jo_paged_layout(const int32_t* cached_lens, const int32_t* new_lens, int32_t
 
 int jo_paged_kv_write(const void* key, const void* value, void* key_cache, void* value_cache, const int64_t* slots,
                       int64_t tokens, int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t page_size,
-                      const int64_t* k_strides, const int64_t* v_strides, const int64_t* kc_strides,
-                      const int64_t* vc_strides, int dtype, void* stream) {
+                      const int64_t* row_strides, const int64_t* cache_strides, int dtype, void* stream) {
   using namespace jo;
   JO_REQUIRE(dtype == JO_DTYPE_BF16 || dtype == JO_DTYPE_F16, JO_ERR_DTYPE, "paged_kv_write: only bf16 and fp16");
   JO_REQUIRE(tokens >= 0 && kv_heads >= 0 && num_blocks >= 0 && page_size >= 1 && tokens < (1LL << 31) &&
@@ -221,10 +220,15 @@ int jo_paged_kv_write(const void* key, const void* value, void* key_cache, void*
   JO_REQUIRE(head_dim >= 8 && head_dim % 8 == 0 && head_dim <= 65536, JO_ERR_INVALID,
              "paged_kv_write: head_dim must be a multiple of 8 (got %lld)", (long long)head_dim);
   if (tokens == 0 || kv_heads == 0 || num_blocks == 0) return JO_OK;
-  JO_REQUIRE(key && value && key_cache && value_cache && slots && k_strides && v_strides && kc_strides && vc_strides,
+  JO_REQUIRE(key && value && key_cache && value_cache && slots && row_strides && cache_strides,
              JO_ERR_INVALID, "paged_kv_write: null pointer");
-  const int64_t all[10] = {k_strides[0],  k_strides[1],  v_strides[0],  v_strides[1],  kc_strides[0],
-                           kc_strides[1], kc_strides[2], vc_strides[0], vc_strides[1], vc_strides[2]};
+  int64_t all[10];
+  for (int i = 0; i < 10; ++i) all[i] = i < 4 ? row_strides[i] : cache_strides[i - 4];
+  // the stride of a dimension of one element is never used
+  if (tokens == 1) all[0] = all[2] = 0;
+  if (kv_heads == 1) all[1] = all[3] = all[6] = all[9] = 0;
+  if (num_blocks == 1) all[4] = all[7] = 0;
+  if (page_size == 1) all[5] = all[8] = 0;
   for (int i = 0; i < 10; ++i)
     JO_REQUIRE(all[i] >= 0 && all[i] % 8 == 0, JO_ERR_ALIGN,
                "paged_kv_write: strides must be non-negative multiples of 8 elements");

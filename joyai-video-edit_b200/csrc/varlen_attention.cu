@@ -10,12 +10,8 @@
 // Organisation of tile_kernel (one block per SM, 384 threads).  The `group`
 // query heads that read one key head are rows of one tile: row r of a tile is
 // token r / group, head r % group, so K and V are read once for all of them.
-// An item is (request, key head, 256 rows as two 128-row tiles); its unit of
-// work is one step over 128 keys.  The units of all items, laid end to end, are
-// cut into one equal range per block, so that ragged lengths and single long
-// requests fill the machine alike; an item that a cut divides leaves partial
-// results (maximum, sum, unnormalised row) that join_kernel adds up in the order
-// of the keys, so results do not depend on timing.
+// An item is (request, key head, 256 rows as two 128-row tiles), a step 128 keys;
+// the steps of all items are shared out evenly (varlen_attention.cuh).
 //   warp 8       TMA producer: Q tiles of an item, K and V of every step (pages
 //                looked up in the block table, one copy per run of a page)
 //   warp 9       MMA issuer: S_t = Q_t K^T, O_t += P_t V on tcgen05, in the order
@@ -30,229 +26,22 @@
 // leave O alone.
 #include <math.h>
 
-#include "sm100_async.cuh"
 #include "varlen_attention.cuh"
 
 namespace jo {
 namespace vattn {
 
-using namespace sm100;
-
 constexpr int kRows = 128;               // rows of a tile
 constexpr int kKeys = 128;               // keys of a step
 constexpr int kThreads = 384;
-constexpr int kMaxBlocks = 256;          // blocks of the tile kernel: one per SM
-constexpr int kScan = 512;               // requests of one scan of the lengths
-// A cut closer than this many steps to an item's edge moves to the edge: a
-// shorter piece would cost more to join than to compute.
-constexpr int kMinPiece = 3;
+constexpr int kLead = 1;                 // steps that an item's beginning and end cost
+constexpr int kMin = 3;                  // steps of the shortest piece
+using Steps = Work<kKeys, kLead, kMin>;
+using Range = Steps::Range;
+using Piece = Steps::Piece;
+using Walk = Steps::Walk;
 
 __device__ int g_fault = 0;
-
-// ------------------------------------------------------------ work ranges --
-// Where block c's range of units lies.
-struct Range {
-  int b, h, qt, tile;                    // first unit; tile may be its item's end
-  long long units;
-};
-
-__device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
-// Steps of item qt: at least one, so that rows that see no key are written too.
-__device__ __forceinline__ int item_units(const Params& p, const Request& r, int qt, int tpt) {
-  const int last = min(r.n, (qt + 1) * 2 * tpt) - 1;
-  return max(1, div_up(visible(p, r, last), kKeys));
-}
-
-struct ScanSpace {
-  int first[kScan], n[kScan], keys[kScan];
-  long long before[kScan + 1];           // units before each request of the scan
-  Range cut[2];
-  long long at[2];
-};
-
-// Range of block c of C.  All threads of the block take part.
-__device__ void find_range(const Params& p, int tpt, int c, int C, ScanSpace& s, Range& range) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int chunks = div_up(p.batch, kScan);
-  long long total = 0, target = 0;
-  // First time round: the number of units.  Second: the places of the cuts.
-  for (int round = 0; round < 2; ++round) {
-    if (round == 1) {
-      target = warp < 2 ? total / C * (c + warp) + total % C * (c + warp) / C : 0;
-      if (warp < 2 && lane == 0) {
-        s.cut[warp] = Range{p.batch, 0, 0, 0, 0};
-        s.at[warp] = total;
-      }
-      __syncwarp();
-    }
-    long long base = 0;
-    for (int ch = 0; ch < chunks; ++ch) {
-      const int cnt = min(kScan, p.batch - ch * kScan);
-      if (round == 0 || chunks > 1) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < cnt; i += kThreads) {
-          const Request r = request(p, ch * kScan + i);
-          s.first[i] = r.first;
-          s.n[i] = r.n;
-          s.keys[i] = r.keys;
-        }
-        __syncthreads();
-        for (int i = warp; i < cnt; i += kThreads / 32) {
-          const Request r{s.first[i], s.n[i], s.keys[i]};
-          const int nq = div_up(r.n, 2 * tpt);
-          long long u = 0;
-          for (int q = lane; q < nq; q += 32) u += item_units(p, r, q, tpt);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-          if (lane == 0) s.before[i + 1] = u * p.kv_heads;
-        }
-        __syncthreads();
-        if (warp == 0) {
-          constexpr int E = kScan / 32;
-          long long mine = 0;
-          for (int i = lane * E; i < min(cnt, lane * E + E); ++i) mine += s.before[i + 1];
-          long long inc = mine;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += x;
-          }
-          long long run = inc - mine;
-          if (lane == 0) s.before[0] = 0;
-          for (int i = lane * E; i < min(cnt, lane * E + E); ++i) {
-            run += s.before[i + 1];
-            s.before[i + 1] = run;
-          }
-        }
-        __syncthreads();
-      }
-      const long long sum = s.before[cnt];
-      if (round == 1 && warp < 2 && target >= base && target < base + sum) {
-        const long long rel = target - base;
-        int a = 0, e = cnt;              // last request that begins at or before rel
-        while (e - a > 1) {
-          const int mid = (a + e) >> 1;
-          if (s.before[mid] <= rel) a = mid; else e = mid;
-        }
-        const Request r{s.first[a], s.n[a], s.keys[a]};
-        const long long per_head = (s.before[a + 1] - s.before[a]) / p.kv_heads;
-        const long long in_req = rel - s.before[a];
-        const int h = (int)(in_req / per_head);
-        long long off = in_req - h * per_head;
-        const int nq = div_up(r.n, 2 * tpt);
-        for (int q0 = 0; q0 < nq; q0 += 32) {
-          const int q = q0 + lane;
-          const long long u = q < nq ? item_units(p, r, q, tpt) : 0;
-          long long inc = u;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += x;
-          }
-          const unsigned hit = __ballot_sync(0xffffffffu, inc > off);
-          if (hit) {
-            if (lane == __ffs(hit) - 1) {
-              long long tile = off - (inc - u), at = target;
-              if (tile < kMinPiece) {
-                at -= tile;
-                tile = 0;
-              } else if (u - tile < kMinPiece) {
-                at += u - tile;
-                tile = u;
-              }
-              s.cut[warp] = Range{ch * kScan + a, h, q, (int)tile, 0};
-              s.at[warp] = at;
-            }
-            break;
-          }
-          off -= __shfl_sync(0xffffffffu, inc, 31);
-        }
-      }
-      base += sum;
-    }
-    total = base;
-  }
-  __syncthreads();
-  range = s.cut[0];
-  range.units = s.at[1] - s.at[0];
-}
-
-// One block's stretch of one item.
-struct Piece {
-  int b, h, qt;
-  Request r;
-  int a, e;                              // steps [a, e) of the item's `units`
-  int units;
-  int end[2];                            // tile t takes part in steps [a, end[t])
-  int edge;                              // first step in which some row does not see every key
-};
-
-// Walks a range piece by piece; every role of a block walks it for itself.
-struct Walk {
-  const Params& p;
-  int tpt, b, h, qt, tile, nq;
-  long long left;
-  Request r;
-  __device__ Walk(const Params& p_, int tpt_, const Range& g)
-      : p(p_), tpt(tpt_), b(g.b), h(g.h), qt(g.qt), tile(g.tile), left(g.units) {
-    if (left > 0) load();
-  }
-  __device__ void load() {
-    r = request(p, b);
-    nq = div_up(r.n, 2 * tpt);
-  }
-  __device__ void advance() {
-    tile = 0;
-    if (++qt < nq) return;
-    qt = 0;
-    if (++h < p.kv_heads) return;
-    h = 0;
-    for (++b; b < p.batch; ++b) {
-      load();
-      if (r.n > 0) return;
-    }
-    left = 0;
-  }
-  __device__ bool next(Piece& s) {
-    while (left > 0) {
-      const int units = item_units(p, r, qt, tpt);
-      if (tile >= units) {
-        advance();
-        continue;
-      }
-      s.b = b;
-      s.h = h;
-      s.qt = qt;
-      s.r = r;
-      s.units = units;
-      s.a = tile;
-      s.e = (int)min((long long)units, tile + left);
-      left -= s.e - s.a;
-      const int tok = qt * 2 * tpt, n = min(2 * tpt, r.n - tok);
-      s.end[0] = max(s.a, min(s.e, max(1, div_up(visible(p, r, tok + min(n, tpt) - 1), kKeys))));
-      s.end[1] = n > tpt ? s.e : s.a;
-      s.edge = visible(p, r, tok) / kKeys;
-      if (left > 0) advance();
-      return true;
-    }
-    return false;
-  }
-};
-
-// ------------------------------------------------------- partial results ----
-// Block c leaves at most two: slot 0 for an item that an earlier block began,
-// slot 1 for one that a later block goes on with.
-struct Piece2Join {
-  int head;      // 0 empty range, 1 slot 0 goes on in a later block, 2 slot 0 ends the item, 3 begins with an item
-  int tail;      // slot 1 holds the beginning of an item
-  int first, n;  // that item's first row (absolute) and its rows' tokens
-  int h;
-  int pad[3];
-};
-template <int D> struct Slot {
-  float o[D / 4][2 * kRows][4];          // column blocks of four, so that a warp's rows are adjacent
-  float2 ml[2 * kRows];                  // maximum, sum
-};
 
 template <int D> struct Cfg {
   static constexpr int HALVES = D / 64;
@@ -270,12 +59,19 @@ struct Maps {
   int tpt;                               // tokens of a tile: 128 / group
   int box;                               // keys of one K or V copy
   void* partial;
-  Piece2Join* join;
+  Begun* begun;
 };
 
-// Byte of element (row, col) of a 128-byte-swizzled tile.
-__device__ __forceinline__ uint32_t swizzled(int row, int col, int half_bytes) {
-  return (col >> 6) * half_bytes + row * 128 + ((((col & 63) * 2) >> 4 ^ (row & 7)) << 4) + ((col & 7) * 2);
+// Steps [s.a, end) of a piece in which tile t takes part: none without rows, and
+// none after the last key that its rows see.
+__device__ __forceinline__ int tile_end(const Params& p, const Piece& s, int tpt, int t) {
+  const int tok = s.i * 2 * tpt, n = min(2 * tpt, s.r.n - tok);
+  if (t == 1) return n > tpt ? s.e : s.a;
+  return max(s.a, min(s.e, max(1, div_up(visible(p, s.r, tok + min(n, tpt) - 1), kKeys))));
+}
+// First step in which some row does not see every key.
+__device__ __forceinline__ int first_edge(const Params& p, const Piece& s, int tpt) {
+  return visible(p, s.r, s.i * 2 * tpt) / kKeys;
 }
 
 // O (+)= P V for one row on the CUDA cores: the step's V holds a NaN or an
@@ -331,7 +127,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   using C = Cfg<D>;
   constexpr int ST = C::ST;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ ScanSpace scan;
+  __shared__ Steps::Scan scan;
+  __shared__ Steps::Near near;
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
@@ -366,14 +163,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   }
   if (warp == 9) tmem_alloc_512(smem_u32(tmem_slot));
   Range range;
-  find_range(p, maps.tpt, blockIdx.x, gridDim.x, scan, range);
+  Steps::find<kThreads>(p, 2 * maps.tpt, blockIdx.x, gridDim.x, scan, near, range);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t sq = smem_u32(smem), sk = sq + C::K0, sv = sq + C::V0;
   const int tpt = maps.tpt;
-  Walk walk(p, tpt, range);
+  Walk walk(p, 2 * tpt, near, range);
   Piece s;
 
   if (warp == 8) {
@@ -391,19 +188,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     }
     uint32_t v_issued = 0;
     while (ok && walk.next(s)) {
+      int z16 = 0, w16 = 0;
       for (int j = s.a; j < s.e && ok; ++j, ++it) {
-        // coordinates of this lane's keys; a block outside the cache reads as zeros
-        int z, w = 0;
-        const int key = j * kKeys + bx * maps.box;
-        if (p.table) {
-          const int pg = key / p.page;
-          z = key - pg * p.page;
-          int block = -1;
-          if (mine && key < s.r.keys) block = p.table[(int64_t)s.b * p.table_stride + pg];
-          w = block >= 0 && block < p.num_blocks ? block : -1;
-        } else {
-          z = s.r.first + key;
-        }
+        // places of 16 keys each, four steps at a time: pages are multiples of 16 keys
+        const int ahead = (j - s.a) & 3;
+        if (ahead == 0) kv_place(p, s.r, s.b, j * kKeys + lane * 16, z16, w16);
+        const int from = (ahead * 8 + bx * (maps.box / 16)) & 31;
+        const int z = __shfl_sync(0xffffffffu, z16, from), w = __shfl_sync(0xffffffffu, w16, from);
         const int st = it % ST;
         const uint32_t ph = (it / ST) & 1;
         ok = WAIT(C::B_KE + st, ph ^ 1, 1);
@@ -417,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             ++it;
             break;
           }
-          const int tok = s.qt * 2 * tpt, tiles = s.r.n - tok > tpt ? 2 : 1;
+          const int tok = s.i * 2 * tpt, tiles = s.r.n - tok > tpt ? 2 : 1;
           if (lane == 0) mbar_expect_tx(BAR(C::B_QF), tiles * D * 2 * p.group * tpt);
           __syncwarp();
           if (lane < tiles * C::HALVES) {
@@ -468,13 +259,16 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       };
       uint32_t it = 0, pieces = 0, seen[2] = {0, 0};
       bool more = walk.next(s), ok = true;
-      int j = s.a;
+      int j = 0, end[2] = {0, 0};
       if (more) {
+        j = s.a;
+        end[0] = tile_end(p, s, tpt, 0);
+        end[1] = tile_end(p, s, tpt, 1);
         ok = WAIT(C::B_QF, 0, 4) && WAIT(C::B_KF, 0, 5);
         if (ok) {
           fence_after();
           for (int t = 0; t < 2; ++t)
-            if (j < s.end[t]) qk(t, 0);
+            if (j < end[t]) qk(t, 0);
           mma_commit(BAR(C::B_KE));
           if (j + 1 == s.e) mma_commit(BAR(C::B_QE));
         }
@@ -483,9 +277,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         Piece ns = s;
         int nj = j + 1;
         const bool turn = nj == s.e;     // the next step begins another piece
+        int nend[2] = {end[0], end[1]};
         if (turn) {
           more = walk.next(ns);
           nj = ns.a;
+          nend[0] = tile_end(p, ns, tpt, 0);
+          nend[1] = tile_end(p, ns, tpt, 1);
           ++pieces;
         }
         const int st = it % ST, nst = (it + 1) % ST;
@@ -493,16 +290,16 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         const bool careful = vflag[2 * st] | vflag[2 * st + 1];
         bool waited = false;
         for (int t = 0; t < 2 && ok; ++t) {
-          if (j < s.end[t]) {
+          if (j < end[t]) {
             ok = WAIT(C::B_PF + t, seen[t] & 1, 7 + t);
             if (!ok) break;
             ++seen[t];
             fence_after();
             if (!careful) pv(t, st, j > s.a);
-            if (j + 1 == s.end[t]) mma_commit(BAR(C::B_OF + t));
+            if (j + 1 == end[t]) mma_commit(BAR(C::B_OF + t));
           }
           if (t == 1) mma_commit(BAR(C::B_VE + st));
-          if (more && nj < ns.end[t]) {
+          if (more && nj < nend[t]) {
             if (!waited) {
               ok = (!turn || WAIT(C::B_QF, pieces & 1, 9)) && WAIT(C::B_KF + nst, ((it + 1) / ST) & 1, 10);
               if (!ok) break;
@@ -519,6 +316,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
         s = ns;
         j = nj;
+        end[0] = nend[0];
+        end[1] = nend[1];
         ++it;
       }
       // Every MMA issued completes before tensor memory is freed.
@@ -530,16 +329,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const int g = warp - 10;
     uint32_t it = 0;
     bool ok = true;
-    Piece2Join jn{range.units > 0 ? 3 : 0, 0, 0, 0, 0, {0, 0, 0}};
+    Begun begun{0, 0, 0, 0};
     while (ok && walk.next(s)) {
-      const int tok = s.qt * 2 * tpt;
-      if (s.a > 0) jn.head = s.e == s.units ? 2 : 1;          // only the first piece begins inside an item
-      if (s.a == 0 && s.e < s.units) {                        // only the last one ends inside one
-        jn.tail = 1;
-        jn.first = s.r.first + tok;
-        jn.n = min(2 * tpt, s.r.n - tok);
-        jn.h = s.h;
-      }
+      const int tok = s.i * 2 * tpt, edge = first_edge(p, s, tpt);
+      if (s.a == 0 && s.e < s.steps)     // only the last piece ends inside an item
+        begun = Begun{Steps::later_blocks(range, s, blockIdx.x), s.r.first + tok, min(2 * tpt, s.r.n - tok), s.h};
       const int some = visible(p, s.r, tok);                                  // seen by every row
       const int most = visible(p, s.r, min(s.r.n, tok + 2 * tpt) - 1);        // seen by any
       for (int j = s.a; j < s.e; ++j, ++it) {
@@ -547,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         ok = __all_sync(0xffffffffu, WAIT(C::B_VF + st, (it / ST) & 1, 11));
         if (!ok) break;
         int bad = 0;
-        if (j >= s.edge) {
+        if (j >= edge) {
           unsigned char* v = smem + C::V0 + st * C::TILE;
           const int lo = max(0, some - j * kKeys), hi = min(kKeys, max(0, most - j * kKeys));
           constexpr int CH = D / 8;      // 16-byte vectors of a row
@@ -573,11 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
       }
     }
-    // what join_kernel needs to know of this block's range
-    if (g == 0 && lane == 0 && maps.join) {
-      if (!ok) jn = Piece2Join{0, 0, 0, 0, 0, {0, 0, 0}};
-      maps.join[blockIdx.x] = jn;
-    }
+    if (g == 0 && lane == 0 && maps.begun) maps.begun[blockIdx.x] = ok ? begun : Begun{0, 0, 0, 0};
   } else {
     // -------------------------------------------------------------- softmax --
     const int t = warp >> 2;                       // tile of this warpgroup
@@ -590,13 +380,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     uint32_t it = 0, tiles = 0, outs = 0;
     bool ok = true;
     while (ok && walk.next(s)) {
-      const int i_tok = s.qt * 2 * tpt + t * tpt + row_tok;
+      const int i_tok = s.i * 2 * tpt + t * tpt + row_tok;
       const bool valid = row_tok < tpt && i_tok < s.r.n;
       const int limit = visible(p, s.r, min(i_tok, s.r.n - 1));
+      const int end = tile_end(p, s, tpt, t), first = first_edge(p, s, tpt);
       float m = kNoMax;                            // running max of s * c (may lag the true one by less than 8)
       float l = 0.f;                               // running sum
       for (int j = s.a; j < s.e; ++j, ++it) {
-        if (j >= s.end[t]) continue;
+        if (j >= end) continue;
         ok = __all_sync(0xffffffffu, WAIT(C::B_SF + t, tiles & 1, 12));
         if (!ok) break;
         ++tiles;
@@ -610,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #pragma unroll
           for (int i = 0; i < 128; ++i) x[i] = -x[i];
         }
-        const bool edge = j >= s.edge;
+        const bool edge = j >= first;
         const int lim = limit - j * kKeys;
         if (edge) {
 #pragma unroll
@@ -674,15 +465,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       }
       if (!ok) break;
       // ---- epilogue ----
-      const bool has = s.end[t] > s.a;
+      const bool has = end > s.a;
       if (has) {
         ok = __all_sync(0xffffffffu, WAIT(C::B_OF + t, outs & 1, 14));
         if (!ok) break;
         ++outs;
         fence_after();
       }
-      const bool whole = s.a == 0 && s.e == s.units;
-      if (whole) {
+      if (s.whole()) {
         if (!has) continue;
         // a row that sees no key has l = 0 and an O that was never scaled: zero
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -708,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           }
         }
       } else {
-        Slot<D>& slot = static_cast<Slot<D>*>(maps.partial)[2 * blockIdx.x + (s.a == 0 ? 1 : 0)];
+        Slot<D, 2 * kRows>& slot = static_cast<Slot<D, 2 * kRows>*>(maps.partial)[2 * blockIdx.x + (s.a == 0 ? 1 : 0)];
         const int r2 = t * kRows + row;
         slot.ml[r2] = make_float2(m, l);
         if (has) {
@@ -736,64 +526,16 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #undef WAIT
 }
 
-// Adds up the partial results of the items that cuts divide.  Block (c, y):
-// the item whose first piece is block c's last; a warp takes 32 rows and 8
-// columns of it (y enumerates them), each lane one row.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) join_kernel(const Params p, const Slot<D>* slots, const Piece2Join* join, int tpt,
-                                                   int blocks) {
-  __shared__ int heads[kMaxBlocks];
-  wait_for_primary();
-  const Piece2Join me = join[blockIdx.x];
-  if (!me.tail) return;
-  for (int i = threadIdx.x; i < blocks; i += blockDim.x) heads[i] = join[i].head;
-  __syncthreads();
-  const int w = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int col = (w % (D / 8)) * 8, r2 = (w / (D / 8)) * 32 + lane;
-  const int t = r2 / kRows, row = r2 % kRows;
-  const int tok_in_tile = row / p.group, tok = t * tpt + tok_in_tile;
-  if (tok_in_tile >= tpt || tok >= me.n) return;
-  float m = kNoMax, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  int c = blockIdx.x, slot = 2 * c + 1;
-  bool last = false;
-  while (true) {
-    const Slot<D>& s = slots[slot];
-    const float2 ml = s.ml[r2];
-    const float4 x = *reinterpret_cast<const float4*>(s.o[col / 4][r2]);
-    const float4 y = *reinterpret_cast<const float4*>(s.o[col / 4 + 1][r2]);
-    if (ml.y != 0.f) {                   // rows without a visible key there have no O either
-      const float mn = fmaxf(m, ml.x), a = ex2(m - mn), b = ex2(ml.x - mn);
-      m = mn;
-      l = l * a + ml.y * b;
-      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = o[i] * a + v[i] * b;
-    }
-    if (last) break;
-    int head = 0;
-    while (++c < blocks && (head = heads[c]) == 0) {
-    }
-    if (c >= blocks || head == 3) break;
-    slot = 2 * c;
-    last = head == 2;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint32_t out[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = pack2<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
-  T* dst = static_cast<T*>(p.out) + (int64_t)(me.first + tok) * p.o_ts + (int64_t)(me.h * p.group + row % p.group) * p.o_hs + col;
-  *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
-}
-
 // ------------------------------------------------------------------- host --
-static int64_t join_bytes(int blocks) { return (int64_t)blocks * (int64_t)sizeof(Piece2Join); }
-static int64_t slot_bytes(int head_dim) {
-  return head_dim == 64 ? (int64_t)sizeof(Slot<64>) : (int64_t)sizeof(Slot<128>);
+static int64_t begun_bytes(int blocks) { return ((int64_t)blocks * (int64_t)sizeof(Begun) + 15) / 16 * 16; }
+static int64_t tile_workspace(int head_dim) {
+  const int n = sm_count();
+  return begun_bytes(n) +
+         2 * (int64_t)n * (int64_t)(head_dim == 64 ? sizeof(Slot<64, 2 * kRows>) : sizeof(Slot<128, 2 * kRows>));
 }
-static int tile_blocks() { return sm_count() < kMaxBlocks ? sm_count() : kMaxBlocks; }
 static int64_t workspace_bytes_for(int head_dim) {
-  const int n = tile_blocks();
-  return join_bytes(n) + 2 * (int64_t)n * slot_bytes(head_dim);
+  const int64_t a = tile_workspace(head_dim), b = few_workspace(head_dim);
+  return a > b ? a : b;
 }
 
 static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
@@ -807,6 +549,12 @@ static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int
   JO_REQUIRE(heads == 0 || (kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= kRows), JO_ERR_INVALID,
              "%s: heads (%lld) must be a multiple of kv_heads (%lld), at most 128 times it", what, (long long)heads,
              (long long)kv_heads);
+  // the stride of a dimension of one element is never used
+  if (tokens <= 1) p.q_ts = p.o_ts = 0;
+  if (tokens <= 1 && !p.table) p.k_ts = p.v_ts = 0;
+  if (heads <= 1) p.q_hs = p.o_hs = 0;
+  if (kv_heads <= 1) p.k_hs = p.v_hs = 0;
+  if (p.num_blocks <= 1) p.k_bs = p.v_bs = 0;
   const int64_t s[10] = {p.q_ts, p.q_hs, p.k_bs, p.k_ts, p.k_hs, p.v_bs, p.v_ts, p.v_hs, p.o_ts, p.o_hs};
   for (int i = 0; i < 10; ++i)
     JO_REQUIRE(s[i] >= 0 && s[i] % 8 == 0, JO_ERR_ALIGN, "%s: strides must be non-negative multiples of 8 elements", what);
@@ -830,35 +578,18 @@ static int launch_tiles(const char* what, const Params& p, void* workspace, cuda
   constexpr bool bf16 = IsBf16<T>::v;
   Maps maps;
   maps.tpt = kRows / p.group;
-  const int blocks = tile_blocks();
+  const int blocks = sm_count();
   const int64_t qd[4] = {D, p.group, p.kv_heads, p.tokens}, qs[3] = {p.q_hs, p.q_hs * p.group, p.q_ts};
   const int qb[4] = {64, p.group, 1, maps.tpt};
-  bool ok = make_map_4d(&maps.q, bf16, p.q, qd, qs, qb);
-  if (p.table) {
-    maps.box = p.page & -p.page;                     // the largest power of two that divides the page
-    if (maps.box > kKeys) maps.box = kKeys;
-    const int kb[4] = {64, 1, maps.box, 1};
-    // an empty cache: every block is outside it, the address is never read
-    const int64_t d[4] = {D, p.kv_heads, p.page, p.num_blocks > 0 ? p.num_blocks : 1};
-    const int64_t ks[3] = {p.k_hs, p.k_ts, p.k_bs}, vs[3] = {p.v_hs, p.v_ts, p.v_bs};
-    ok = ok && make_map_4d(&maps.k, bf16, p.num_blocks > 0 ? p.k : p.q, d, ks, kb) &&
-         make_map_4d(&maps.v, bf16, p.num_blocks > 0 ? p.v : p.q, d, vs, kb);
-  } else {
-    maps.box = kKeys;
-    const int kb[4] = {64, 1, kKeys, 1};
-    const int64_t d[4] = {D, p.kv_heads, p.tokens, 1};
-    const int64_t ks[3] = {p.k_hs, p.k_ts, 0}, vs[3] = {p.v_hs, p.v_ts, 0};
-    ok = ok && make_map_4d(&maps.k, bf16, p.k, d, ks, kb) && make_map_4d(&maps.v, bf16, p.v, d, vs, kb);
-  }
-  if (!ok) {
+  if (!make_map_4d(&maps.q, bf16, p.q, qd, qs, qb) || !kv_maps(p, bf16, kKeys, &maps.k, &maps.v, &maps.box)) {
     set_error("%s: cuTensorMapEncodeTiled failed", what);
     return JO_ERR_CUDA;
   }
   // No item has a cut inside when none is long enough to have one away from its edges.
   const int64_t most_keys = p.table ? (int64_t)p.width * p.page : p.tokens;
-  const bool split = most_keys > (2 * kMinPiece - 1) * kKeys;
-  maps.join = split ? static_cast<Piece2Join*>(workspace) : nullptr;
-  maps.partial = static_cast<char*>(workspace) + join_bytes(blocks);
+  const bool split = most_keys > (2 * kMin - 1) * kKeys;
+  maps.begun = split ? static_cast<Begun*>(workspace) : nullptr;
+  maps.partial = static_cast<char*>(workspace) + begun_bytes(blocks);
   static bool attr[kMaxDevices] = {};
   const int dev = device_slot();
   if (!attr[dev]) {
@@ -867,23 +598,20 @@ static int launch_tiles(const char* what, const Params& p, void* workspace, cuda
     attr[dev] = true;
   }
   tile_kernel<T, D><<<blocks, kThreads, Cfg<D>::BYTES, stream>>>(maps, p);
-  if (split) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks, 2 * kRows / 32 * (D / 8) / 8);
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p, static_cast<const Slot<D>*>(maps.partial),
-                       static_cast<const Piece2Join*>(maps.join), maps.tpt, blocks);
-  }
+  if (split) launch_join<T, D, 2 * kRows, kRows, 1>(p, maps.partial, maps.begun, maps.tpt, blocks, stream);
   return check_launch(what);
 }
 
-static int launch(const char* what, const Params& p, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+static int launch_all_tiles(const char* what, const Params& p, int dtype, void* workspace, cudaStream_t s) {
+  if (dtype == JO_DTYPE_BF16)
+    return p.head_dim == 64 ? launch_tiles<__nv_bfloat16, 64>(what, p, workspace, s)
+                            : launch_tiles<__nv_bfloat16, 128>(what, p, workspace, s);
+  return p.head_dim == 64 ? launch_tiles<__half, 64>(what, p, workspace, s)
+                          : launch_tiles<__half, 128>(what, p, workspace, s);
+}
+
+static int launch(const char* what, Params& p, int64_t max_query_len, int dtype, void* workspace,
+                  int64_t workspace_bytes, void* stream) {
   if (p.tokens == 0 || p.batch == 0 || p.heads == 0) return JO_OK;
   JO_REQUIRE(p.q && p.out && p.starts, JO_ERR_INVALID, "%s: null tensor pointer", what);
   int st = require_sm100();
@@ -893,11 +621,24 @@ static int launch(const char* what, const Params& p, int dtype, void* workspace,
              "%s: a 16-byte aligned workspace of %lld bytes is needed (got %lld)", what, (long long)need,
              (long long)workspace_bytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == JO_DTYPE_BF16)
-    return p.head_dim == 64 ? launch_tiles<__nv_bfloat16, 64>(what, p, workspace, s)
-                            : launch_tiles<__nv_bfloat16, 128>(what, p, workspace, s);
-  return p.head_dim == 64 ? launch_tiles<__half, 64>(what, p, workspace, s)
-                          : launch_tiles<__half, 128>(what, p, workspace, s);
+  // A request of few rows is bound by reading its keys and is served by its own
+  // kernel.  Where the longest request is one, that kernel takes them all (in
+  // runs of rows, should one be longer than announced); where a batch may hold
+  // both kinds, each kernel takes its own.
+  p.min_rows = 1;
+  p.max_rows = INT32_MAX;
+  if (!p.table) return launch_all_tiles(what, p, dtype, workspace, s);
+  const int64_t longest = max_query_len < p.tokens ? (max_query_len > 1 ? max_query_len : 1) : p.tokens;
+  if (p.group <= kFewRows && longest * p.group <= kFewRows)
+    return launch_few(what, p, longest * p.group, dtype, workspace, s);
+  if (p.group <= kFewRows && p.batch > 1) {
+    p.max_rows = kFewRows;
+    st = launch_few(what, p, kFewRows, dtype, workspace, s);
+    if (st != JO_OK) return st;
+    p.min_rows = kFewRows + 1;
+    p.max_rows = INT32_MAX;
+  }
+  return launch_all_tiles(what, p, dtype, workspace, s);
 }
 
 }  // namespace vattn
@@ -908,20 +649,20 @@ extern "C" {
 int jo_paged_attention(const void* q, const void* key_cache, const void* value_cache, const int32_t* block_tables,
                        const int32_t* query_starts, const int32_t* kv_lens, void* out, int64_t tokens, int64_t batch,
                        int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t page_size,
-                       int64_t table_width, int64_t table_stride, const int64_t* q_strides, const int64_t* kc_strides,
-                       const int64_t* vc_strides, const int64_t* o_strides, int causal, float scale,
-                       int64_t max_query_len, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+                       int64_t table_width, int64_t table_stride, const int64_t* row_strides,
+                       const int64_t* cache_strides, int causal, float scale, int64_t max_query_len, int dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace jo;
   const char* what = "paged_attention";
-  JO_REQUIRE(q_strides && kc_strides && vc_strides && o_strides, JO_ERR_INVALID, "%s: null strides", what);
+  JO_REQUIRE(row_strides && cache_strides, JO_ERR_INVALID, "%s: null strides", what);
+  const int64_t *r = row_strides, *c = cache_strides;
   JO_REQUIRE(page_size >= 16 && page_size % 16 == 0 && page_size < (1LL << 30), JO_ERR_INVALID,
              "%s: page_size must be a multiple of 16 (got %lld)", what, (long long)page_size);
   JO_REQUIRE(num_blocks >= 0 && num_blocks < (1LL << 31) && table_width >= 0 && table_width < (1LL << 31) &&
                  table_stride >= 0 && table_width * page_size < (1LL << 31),
              JO_ERR_INVALID, "%s: invalid cache or block table shape", what);
   vattn::Params p{q, key_cache, value_cache, out, query_starts, kv_lens, block_tables,
-                  q_strides[0], q_strides[1], kc_strides[0], kc_strides[1], kc_strides[2],
-                  vc_strides[0], vc_strides[1], vc_strides[2], o_strides[0], o_strides[1], table_stride};
+                  r[0], r[1], c[0], c[1], c[2], c[3], c[4], c[5], r[2], r[3], table_stride};
   p.num_blocks = (int)num_blocks;
   p.page = (int)page_size;
   p.width = (int)table_width;
@@ -930,20 +671,18 @@ int jo_paged_attention(const void* q, const void* key_cache, const void* value_c
   if (st != JO_OK) return st;
   JO_REQUIRE(tokens == 0 || batch == 0 || (kv_lens && block_tables && (num_blocks == 0 || (key_cache && value_cache))),
              JO_ERR_INVALID, "%s: null tensor pointer", what);
-  (void)max_query_len;
-  return vattn::launch(what, p, dtype, workspace, workspace_bytes, stream);
+  return vattn::launch(what, p, max_query_len, dtype, workspace, workspace_bytes, stream);
 }
 
 int jo_prompt_attention(const void* q, const void* k, const void* v, const int32_t* seq_starts, void* out,
                         int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                        const int64_t* o_strides, int causal, float scale, int dtype, void* workspace,
-                        int64_t workspace_bytes, void* stream) {
+                        const int64_t* row_strides, const int64_t* kv_strides, int causal, float scale, int dtype,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace jo;
   const char* what = "prompt_attention";
-  JO_REQUIRE(q_strides && k_strides && v_strides && o_strides, JO_ERR_INVALID, "%s: null strides", what);
-  vattn::Params p{q, k, v, out, seq_starts, nullptr, nullptr, q_strides[0], q_strides[1], 0, k_strides[0], k_strides[1],
-                  0, v_strides[0], v_strides[1], o_strides[0], o_strides[1], 0};
+  JO_REQUIRE(row_strides && kv_strides, JO_ERR_INVALID, "%s: null strides", what);
+  const int64_t *r = row_strides, *c = kv_strides;
+  vattn::Params p{q, k, v, out, seq_starts, nullptr, nullptr, r[0], r[1], 0, c[0], c[1], 0, c[2], c[3], r[2], r[3], 0};
   p.num_blocks = 0;
   p.page = 1;
   p.width = 0;
@@ -951,7 +690,7 @@ int jo_prompt_attention(const void* q, const void* k, const void* v, const int32
   int st = vattn::check(what, p, tokens, batch, heads, kv_heads, head_dim, scale, dtype);
   if (st != JO_OK) return st;
   JO_REQUIRE(tokens == 0 || batch == 0 || (k && v), JO_ERR_INVALID, "%s: null tensor pointer", what);
-  return vattn::launch(what, p, dtype, workspace, workspace_bytes, stream);
+  return vattn::launch(what, p, tokens, dtype, workspace, workspace_bytes, stream);
 }
 
 int jo_varlen_attention_workspace(int64_t tokens, int64_t heads, int64_t head_dim, int64_t* bytes) {
@@ -976,7 +715,8 @@ int jo_varlen_attention_last_fault(int reset) {
     int z = 0;
     cudaMemcpyToSymbol(jo::vattn::g_fault, &z, sizeof(int));
   }
-  return v;
+  const int w = jo::vattn::few_last_fault(reset);
+  return v != 0 ? v : w;
 }
 
 }  // extern "C"

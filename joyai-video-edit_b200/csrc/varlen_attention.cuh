@@ -1,11 +1,21 @@
 // What the kernels of the variable-length attention share: the arguments, the
-// requests' lengths, and the partial results of work that is split along the keys.
+// division of the work over blocks, and the joining of partial results.
+//
+// An item is (request, key head, a run of the request's rows); its unit of work
+// is one step over a fixed number of keys.  The units of all items, laid end to
+// end in the order (request, key head, rows), are cut into one range per block,
+// all of the same length, so that ragged lengths and single long requests fill
+// the machine alike.  An item that a cut divides leaves partial results
+// (maximum, sum, unnormalised rows), which join_kernel adds up in the order of
+// the keys: results do not depend on timing.
 #pragma once
 
-#include "jo_common.cuh"
+#include "sm100_async.cuh"
 
 namespace jo {
 namespace vattn {
+
+using namespace sm100;
 
 // Strides in elements.
 struct Params {
@@ -20,10 +30,12 @@ struct Params {
   int tokens, batch, heads, kv_heads, group, head_dim, num_blocks, page, width, causal;
   float scale_log2;             // |scale| * log2(e), never 0
   int negate;                   // scale < 0
+  // Which requests a kernel takes, by their rows (tokens * group).
+  int min_rows, max_rows;
 };
 
-// Rows [first, first + n) and keys of request b.  Lengths are device data and
-// are clamped to what the tensors hold.
+// Rows [first, first + n) and keys of request b; n = 0 for one that this kernel
+// does not take.  Lengths are device data and are clamped to what the tensors hold.
 struct Request {
   int first, n, keys;
 };
@@ -32,6 +44,8 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   r.first = min(max(p.starts[b], 0), p.tokens);
   r.n = min(max(p.starts[b + 1], r.first), p.tokens) - r.first;
   r.keys = p.kv_lens ? (int)min((long long)max(p.kv_lens[b], 0), (long long)p.width * p.page) : r.n;
+  const long long rows = (long long)r.n * p.group;
+  if (rows < p.min_rows || rows > p.max_rows) r.n = 0;
   return r;
 }
 // Keys that row i of the request sees.
@@ -40,9 +54,427 @@ __device__ __forceinline__ int visible(const Params& p, const Request& r, int i)
 }
 
 // Running maxima (of scale * log2(e) * s) start here instead of at -infinity, so
-// that a tile in which a row sees no key leaves exp2(0) = 1 and exp2(-inf) = 0,
+// that a step in which a row sees no key leaves exp2(0) = 1 and exp2(-inf) = 0,
 // and no NaN.
 constexpr float kNoMax = -1e30f;
+
+__host__ __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
+
+constexpr int kScan = 512;               // requests of one scan of the lengths
+
+constexpr int kNear = 32;                // requests of a block's range that it keeps at hand
+
+// KEYS keys of a step.  Beginning and ending an item costs as much as LEAD steps,
+// which count as units of work too.  A cut closer than MIN steps to an item's
+// edge moves to the edge: a shorter piece would cost more to join than to compute.
+template <int KEYS, int LEAD, int MIN>
+struct Work {
+  // Steps of item i: at least one, so that rows that see no key are written too.
+  static __device__ __forceinline__ int steps(const Params& p, const Request& r, int i, int tpi) {
+    const int last = (int)min((long long)r.n, (i + 1LL) * tpi) - 1;
+    return max(1, div_up(visible(p, r, last), KEYS));
+  }
+  static __device__ __forceinline__ int units(const Params& p, const Request& r, int i, int tpi) {
+    return LEAD + steps(p, r, i, tpi);
+  }
+
+  // Where a block's range of units lies.
+  struct Range {
+    int b, h, i, step;                   // its first step, which may be its item's end
+    int blocks;                          // ranges that are not empty by intent
+    long long begin, end, total;
+  };
+  // The range's requests, as far as they have room: every role of the block
+  // walks over them, and a look at the lengths in global memory for each would
+  // cost as much as a short request itself.
+  struct Near {
+    int count, next;                     // requests kept; where the ones after them begin
+    int b[kNear];
+    Request r[kNear];
+  };
+  static __device__ __forceinline__ long long cut_at(long long total, int blocks, int c) {
+    return c >= blocks ? total : total / blocks * c + total % blocks * c / blocks;
+  }
+
+  struct Scan {
+    int first[kScan], n[kScan], keys[kScan];
+    long long before[kScan + 1];         // units before each request of the scan
+    Range cut[2];
+    long long at[2];
+  };
+
+  // Range of block c of at most C.  All THREADS threads of the block take part.
+  template <int THREADS>
+  static __device__ void find(const Params& p, int tpi, int c, int C, Scan& s, Near& near, Range& range) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int chunks = div_up(p.batch, kScan);
+    long long total = 0, target = 0;
+    int blocks = C;
+    // First time round: the number of units.  Second: the places of the cuts.
+    for (int round = 0; round < 2; ++round) {
+      if (round == 1) {
+        blocks = (int)max(1LL, min((long long)C, total / (MIN + LEAD)));
+        target = warp < 2 ? cut_at(total, blocks, c + warp) : total;
+        if (warp < 2 && lane == 0) {
+          s.cut[warp] = Range{p.batch, 0, 0, 0, 0, 0, 0, 0};
+          s.at[warp] = total;
+        }
+        __syncwarp();
+      }
+      long long base = 0;
+      for (int ch = 0; ch < chunks; ++ch) {
+        const int cnt = min(kScan, p.batch - ch * kScan);
+        if (round == 0 || chunks > 1) {
+          __syncthreads();
+          for (int i = threadIdx.x; i < cnt; i += THREADS) {
+            const Request r = request(p, ch * kScan + i);
+            s.first[i] = r.first;
+            s.n[i] = r.n;
+            s.keys[i] = r.keys;
+          }
+          __syncthreads();
+          for (int i = warp; i < cnt; i += THREADS / 32) {
+            const Request r{s.first[i], s.n[i], s.keys[i]};
+            const int ni = div_up(r.n, tpi);
+            long long u = 0;
+            for (int q = lane; q < ni; q += 32) u += units(p, r, q, tpi);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+            if (lane == 0) s.before[i + 1] = u * p.kv_heads;
+          }
+          __syncthreads();
+          if (warp == 0) {
+            constexpr int E = kScan / 32;
+            long long mine = 0;
+            for (int i = lane * E; i < min(cnt, lane * E + E); ++i) mine += s.before[i + 1];
+            long long inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+              if (lane >= o) inc += x;
+            }
+            long long run = inc - mine;
+            if (lane == 0) s.before[0] = 0;
+            for (int i = lane * E; i < min(cnt, lane * E + E); ++i) {
+              run += s.before[i + 1];
+              s.before[i + 1] = run;
+            }
+          }
+          __syncthreads();
+        }
+        const long long sum = s.before[cnt];
+        if (round == 1 && warp < 2 && target >= base && target < base + sum) {
+          const long long rel = target - base;
+          int a = 0, e = cnt;            // last request that begins at or before rel
+          while (e - a > 1) {
+            const int mid = (a + e) >> 1;
+            if (s.before[mid] <= rel) a = mid; else e = mid;
+          }
+          const Request r{s.first[a], s.n[a], s.keys[a]};
+          const long long per_head = (s.before[a + 1] - s.before[a]) / p.kv_heads;
+          const long long in_req = rel - s.before[a];
+          const int h = (int)(in_req / per_head);
+          long long off = in_req - h * per_head;
+          const int ni = div_up(r.n, tpi);
+          for (int q0 = 0; q0 < ni; q0 += 32) {
+            const int q = q0 + lane;
+            const long long u = q < ni ? units(p, r, q, tpi) : 0;
+            long long inc = u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+              if (lane >= o) inc += x;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, inc > off);
+            if (hit) {
+              if (lane == __ffs(hit) - 1) {
+                long long step = off - (inc - u) - LEAD, at = target;
+                const long long last = u - LEAD;
+                if (step < MIN) {
+                  at -= step + LEAD;
+                  step = 0;
+                } else if (last - step < MIN) {
+                  at += last - step;
+                  step = last;
+                }
+                s.cut[warp] = Range{ch * kScan + a, h, q, (int)step, 0, 0, 0, 0};
+                s.at[warp] = at;
+              }
+              break;
+            }
+            off -= __shfl_sync(0xffffffffu, inc, 31);
+          }
+        }
+        base += sum;
+      }
+      total = base;
+    }
+    __syncthreads();
+    range = s.cut[0];
+    range.blocks = blocks;
+    range.begin = s.at[0];
+    range.end = s.at[1];
+    range.total = total;
+    const int last = min(s.cut[1].b, p.batch - 1);
+    if (warp == 0) {
+      int count = 0, b0 = range.b;
+      for (; b0 <= last && count < kNear; b0 += 32) {
+        Request r{0, 0, 0};
+        if (b0 + lane <= last) r = request(p, b0 + lane);
+        const unsigned any = __ballot_sync(0xffffffffu, r.n > 0);
+        const int at = count + __popc(any & ((1u << lane) - 1));
+        if (r.n > 0 && at < kNear) {
+          near.b[at] = b0 + lane;
+          near.r[at] = r;
+        }
+        count += __popc(any);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        near.count = min(count, kNear);
+        near.next = count > kNear ? near.b[kNear - 1] + 1 : b0;
+      }
+    }
+  }
+
+  // One block's stretch of one item.
+  struct Piece {
+    int b, h, i;
+    Request r;
+    int a, e;                            // steps [a, e) of the item's `steps`
+    int steps;
+    long long at;                        // unit at which the item's steps begin
+    __device__ bool whole() const { return a == 0 && e == steps; }
+  };
+
+  // Walks a range piece by piece; every role of a block walks it for itself.
+  struct Walk {
+    const Params& p;
+    const Near& near;
+    int tpi, k, b, h, i, step, ni;
+    long long at, end;
+    Request r;
+    // (The range's first request is the first of the near ones: it has rows.)
+    __device__ Walk(const Params& p_, int tpi_, const Near& near_, const Range& g)
+        : p(p_), near(near_), tpi(tpi_), k(0), b(g.b), h(g.h), i(g.i), step(g.step), at(g.begin), end(g.end) {
+      if (at < end) {
+        r = near.r[0];
+        ni = div_up(r.n, tpi);
+      }
+    }
+    __device__ void advance() {
+      step = 0;
+      if (++i < ni) return;
+      i = 0;
+      if (++h < p.kv_heads) return;
+      h = 0;
+      if (++k < near.count) {
+        b = near.b[k];
+        r = near.r[k];
+      } else {
+        b = k == near.count ? near.next : b + 1;
+        r.n = 0;
+        for (; b < p.batch; ++b) {
+          r = request(p, b);
+          if (r.n > 0) break;
+        }
+        if (r.n == 0) at = end;
+      }
+      ni = div_up(r.n, tpi);
+    }
+    __device__ bool next(Piece& s) {
+      while (at < end) {
+        const int n = Work::steps(p, r, i, tpi);
+        if (step >= n) {
+          advance();
+          continue;
+        }
+        if (step == 0) at += LEAD;
+        s.b = b;
+        s.h = h;
+        s.i = i;
+        s.r = r;
+        s.steps = n;
+        s.a = step;
+        s.e = (int)min((long long)n, step + max(1LL, end - at));
+        s.at = at - step;
+        at += s.e - s.a;
+        if (at < end) advance();
+        return true;
+      }
+      return false;
+    }
+  };
+
+  // Blocks after this one that have a piece of the item that piece s begins.
+  static __device__ int later_blocks(const Range& g, const Piece& s, int c) {
+    // block c' has one if its cut is not past the item's end, nor so close to it that it moved there
+    const long long x = s.at + s.steps - MIN;
+    int last = (int)min((long long)g.blocks - 1, (x + 1) * g.blocks / g.total);
+    while (last + 1 < g.blocks && cut_at(g.total, g.blocks, last + 1) <= x) ++last;
+    while (last > c && cut_at(g.total, g.blocks, last) > x) --last;
+    return last - c;
+  }
+};
+
+// ------------------------------------------------------- partial results ----
+// Block c leaves at most two: slot 0 for an item that an earlier block began,
+// slot 1 for one that later blocks go on with.
+struct Begun {
+  int later;     // blocks that go on with the item in slot 1; 0: no such item
+  int first, n;  // its first row's token (absolute) and its tokens
+  int h;
+};
+// R rows in column blocks of four, so that the rows of a warp are adjacent.
+template <int D, int R> struct Slot {
+  float o[D / 4][R][4];
+  float2 ml[R];                          // maximum, sum
+};
+
+// Token and head of row r of an item whose rows come in tiles of TILE rows, tpt tokens each.
+template <int TILE>
+__device__ __forceinline__ bool row_place(int r, int group, int tpt, int n, int& tok, int& head) {
+  const int t = r / TILE, in = r - t * TILE, k = in / group;
+  tok = t * tpt + k;
+  head = in - k * group;
+  return k < tpt && tok < n;
+}
+
+// Adds up the partial results of the items that cuts divide.  Block (c, y): the
+// item that block c of the attention kernel began and did not end.  A team of
+// TEAM warps takes 32 rows and 8 columns of it (y and the team's place in the
+// block enumerate them), each lane one row; the team's warps share out the
+// partial results and warp 0 adds theirs up.  Latency-bound: the reads of four
+// partial results are in flight at a time.
+template <typename T, int D, int R, int TILE, int TEAM>
+__global__ void __launch_bounds__(256) join_kernel(const Params p, const Slot<D, R>* slots, const Begun* begun, int tpt) {
+  static_assert(8 % TEAM == 0, "");
+  __shared__ float shared[TEAM > 1 ? 8 : 1][10][32];
+  wait_for_primary();
+  const int c = blockIdx.x;
+  const Begun me = begun[c];
+  if (me.later == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp % TEAM;
+  const int w = blockIdx.y * (8 / TEAM) + warp / TEAM;
+  const int col = (w % (D / 8)) * 8, r = (w / (D / 8)) * 32 + lane;
+  int tok, head;
+  const bool valid = row_place<TILE>(r, p.group, tpt, me.n, tok, head);
+  float m = kNoMax, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int count = me.later + 1;        // slots 2c+1, 2c+2, 2c+4, ..., 2(c+later)
+  const int per = (count + TEAM - 1) / TEAM, lo = member * per, hi = min(count, lo + per);
+  for (int i0 = lo; i0 < hi; i0 += 4) {
+    float2 ml[4];
+    float4 x[4], y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = min(i0 + k, hi - 1);
+      const Slot<D, R>& s = slots[i == 0 ? 2 * c + 1 : 2 * (c + i)];
+      ml[k] = s.ml[r];
+      x[k] = *reinterpret_cast<const float4*>(s.o[col / 4][r]);
+      y[k] = *reinterpret_cast<const float4*>(s.o[col / 4 + 1][r]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i0 + k >= hi || ml[k].y == 0.f) continue;      // a row without a visible key there has no O either
+      const float mn = fmaxf(m, ml[k].x), a = ex2(m - mn), b = ex2(ml[k].x - mn);
+      m = mn;
+      l = l * a + ml[k].y * b;
+      const float v[8] = {x[k].x, x[k].y, x[k].z, x[k].w, y[k].x, y[k].y, y[k].z, y[k].w};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) o[q] = o[q] * a + v[q] * b;
+    }
+  }
+  if (TEAM > 1) {
+    float(*mine)[32] = shared[warp];
+    mine[0][lane] = m;
+    mine[1][lane] = l;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) mine[2 + q][lane] = o[q];
+    __syncthreads();
+    if (member != 0) return;
+    for (int k = 1; k < TEAM; ++k) {
+      float(*other)[32] = shared[warp + k];
+      if (other[1][lane] == 0.f) continue;
+      const float mo = other[0][lane], mn = fmaxf(m, mo), a = ex2(m - mn), b = ex2(mo - mn);
+      m = mn;
+      l = l * a + other[1][lane] * b;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) o[q] = o[q] * a + other[2 + q][lane] * b;
+    }
+  }
+  if (!valid) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint4 out;
+  out.x = pack2<T>(o[0] * inv, o[1] * inv);
+  out.y = pack2<T>(o[2] * inv, o[3] * inv);
+  out.z = pack2<T>(o[4] * inv, o[5] * inv);
+  out.w = pack2<T>(o[6] * inv, o[7] * inv);
+  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)(me.first + tok) * p.o_ts +
+                            (int64_t)(me.h * p.group + head) * p.o_hs + col) = out;
+}
+
+template <typename T, int D, int R, int TILE, int TEAM>
+inline void launch_join(const Params& p, const void* slots, const Begun* begun, int tpt, int blocks, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks, R / 32 * (D / 8) / (8 / TEAM));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, join_kernel<T, D, R, TILE, TEAM>, p, static_cast<const Slot<D, R>*>(slots), begun, tpt);
+}
+
+// ----------------------------------------------------------- K and V maps ----
+// Byte of element (row, col) of a 128-byte-swizzled tile whose 64-column blocks
+// are half_bytes apart.
+__device__ __forceinline__ uint32_t swizzled(int row, int col, int half_bytes) {
+  return (col >> 6) * half_bytes + row * 128 + ((((col & 63) * 2) >> 4 ^ (row & 7)) << 4) + ((col & 7) * 2);
+}
+
+// Maps of K and V for copies of `box` keys of one head: the largest power of two
+// that divides the page, so that no copy crosses one, up to `most`.
+inline bool kv_maps(const Params& p, bool bf16, int most, CUtensorMap* k, CUtensorMap* v, int* box) {
+  if (p.table) {
+    *box = p.page & -p.page;
+    if (*box > most) *box = most;
+    const int kb[4] = {64, 1, *box, 1};
+    // an empty cache: every block is outside it, the address is never read
+    const int64_t d[4] = {p.head_dim, p.kv_heads, p.page, p.num_blocks > 0 ? p.num_blocks : 1};
+    const int64_t ks[3] = {p.k_hs, p.k_ts, p.k_bs}, vs[3] = {p.v_hs, p.v_ts, p.v_bs};
+    return make_map_4d(k, bf16, p.num_blocks > 0 ? p.k : p.q, d, ks, kb) &&
+           make_map_4d(v, bf16, p.num_blocks > 0 ? p.v : p.q, d, vs, kb);
+  }
+  *box = most;
+  const int kb[4] = {64, 1, most, 1};
+  const int64_t d[4] = {p.head_dim, p.kv_heads, p.tokens, 1};
+  const int64_t ks[3] = {p.k_hs, p.k_ts, 0}, vs[3] = {p.v_hs, p.v_ts, 0};
+  return make_map_4d(k, bf16, p.k, d, ks, kb) && make_map_4d(v, bf16, p.v, d, vs, kb);
+}
+
+// Coordinates (z, w) of key `key` in those maps; a block outside the cache, and
+// a key past the request's, read as zeros.
+__device__ __forceinline__ void kv_place(const Params& p, const Request& r, int b, int key, int& z, int& w) {
+  if (p.table) {
+    const int pg = key / p.page;
+    z = key - pg * p.page;
+    int block = -1;
+    if (key < r.keys) block = p.table[(int64_t)b * p.table_stride + pg];
+    w = block >= 0 && block < p.num_blocks ? block : -1;
+  } else {
+    z = r.first + key;
+    w = 0;
+  }
+}
+
+// The kernel for requests of few rows (varlen_few.cu): rows, the most of any
+// request as far as the host knows it; up to kFewRows it serves them best.
+constexpr int kFewRows = 32;
+int64_t few_workspace(int head_dim);
+int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, cudaStream_t stream);
+int few_last_fault(int reset);
 
 }  // namespace vattn
 }  // namespace jo

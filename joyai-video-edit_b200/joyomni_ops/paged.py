@@ -27,8 +27,15 @@ from . import _lib
 from ._lib import check as _check, lib as _L
 
 _DT16 = {torch.float16: _lib.JO_DTYPE_F16, torch.bfloat16: _lib.JO_DTYPE_BF16}
-_S2 = ctypes.c_int64 * 2
-_S3 = ctypes.c_int64 * 3
+_I32, _I64 = torch.int32, torch.int64
+_S4 = ctypes.c_int64 * 4
+_S6 = ctypes.c_int64 * 6
+_stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice
+
+# These calls take a few microseconds on the GPU, so what the host does for one
+# counts: arguments are looked at in one expression each, and only a refusal
+# walks through them again to say what is wrong (_refuse_*).
 
 
 def _chk(cond: bool, msg: str) -> None:
@@ -37,30 +44,36 @@ def _chk(cond: bool, msg: str) -> None:
 
 
 class _On:
-    """Makes the tensor's device current where it is not, and gives its current stream."""
+    """Makes device `idx` current for a call and gives its current stream."""
 
-    __slots__ = ("dev", "prev")
+    __slots__ = ("idx", "prev")
 
-    def __init__(self, t: torch.Tensor):
-        self.dev = t.device.index
-        self.prev = None
+    def __init__(self, idx: int):
+        self.idx = idx
 
     def __enter__(self) -> int:
-        cur = torch.cuda.current_device()
-        if cur != self.dev:
-            self.prev = cur
-            torch.cuda.set_device(self.dev)
-        return torch.cuda.current_stream(self.dev).cuda_stream
+        self.prev = _device()
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.idx)
+        return _stream(self.idx)
 
     def __exit__(self, *exc):
-        if self.prev is not None:
+        if self.prev != self.idx:
             torch.cuda.set_device(self.prev)
         return False
 
 
-def _ints(t: torch.Tensor, name: str, dim: int, dtype: torch.dtype, dev) -> None:
-    _chk(t.is_cuda and t.device == dev, f"{name} must be a CUDA tensor on {dev}")
-    _chk(t.dtype == dtype and t.dim() == dim, f"{name} must be a {dim}-D {dtype} tensor")
+def _ints(t: torch.Tensor, name: str, dim: int, dtype: torch.dtype, idx: int) -> None:
+    _chk(t.is_cuda, f"{name} must be a CUDA tensor")
+    _chk(t.get_device() == idx, f"{name} must be on cuda:{idx}")
+    _chk(t.dtype is dtype and t.dim() == dim, f"{name} must be a {dim}-D {dtype} tensor")
+    _chk(t.numel() <= 1 or t.stride(-1) == 1, f"{name} last dim must be contiguous")
+
+
+def _rows(t: torch.Tensor, name: str, dtype, idx: int) -> None:
+    _chk(t.is_cuda, f"{name} must be a CUDA tensor")
+    _chk(t.get_device() == idx, f"{name} must be on cuda:{idx}")
+    _chk(t.dtype is dtype, f"{name} dtype is {t.dtype}, expected {dtype}")
     _chk(t.numel() == 0 or t.stride(-1) == 1, f"{name} last dim must be contiguous")
 
 
@@ -92,35 +105,45 @@ def paged_layout(cached_lens, new_lens, block_tables, free_blocks, page_size: in
     request get slot -1 and position 0.  Where the free list or a table row is too
     short the slot is -1, and ``blocks_needed`` tells how many blocks the step
     wanted.  out: a PagedLayout to write into (its tensors contiguous)."""
-    dev = cached_lens.device
-    for t, n in ((cached_lens, "cached_lens"), (new_lens, "new_lens"), (free_blocks, "free_blocks")):
-        _ints(t, n, 1, torch.int32, dev)
-    _ints(block_tables, "block_tables", 2, torch.int32, dev)
-    B, width = block_tables.shape
-    _chk(cached_lens.size(0) == B and new_lens.size(0) == B, "cached_lens, new_lens and block_tables must have a row "
-                                                             "per request")
-    _chk(num_tokens >= 0, "num_tokens must not be negative")
-    stride = block_tables.stride(0) if B > 1 else width
+    idx = cached_lens.get_device()
+    B = cached_lens.numel()
+    if not (idx >= 0 and cached_lens.dtype is _I32 and new_lens.dtype is _I32 and free_blocks.dtype is _I32
+            and block_tables.dtype is _I32 and new_lens.get_device() == idx and free_blocks.get_device() == idx
+            and block_tables.get_device() == idx and cached_lens.dim() == new_lens.dim() == free_blocks.dim() == 1
+            and cached_lens.is_contiguous() and new_lens.is_contiguous() and free_blocks.is_contiguous()
+            and block_tables.dim() == 2 and block_tables.is_contiguous() and block_tables.size(0) == B
+            and new_lens.numel() == B and num_tokens >= 0):
+        _refuse_layout(cached_lens, new_lens, block_tables, free_blocks, num_tokens)
+    width = block_tables.size(1)
     if out is None:
-        out = PagedLayout.empty(B, num_tokens, dev)
-    else:
-        want = ((B + 1, torch.int32), (B, torch.int32), (num_tokens, torch.int64), (num_tokens, torch.int32),
-                (1, torch.int32))
-        for t, (n, dt), name in zip(out, want, PagedLayout._fields):
-            _chk(t.device == dev and t.dtype == dt and t.shape == (n,) and t.is_contiguous(),
-                 f"out.{name} must be a contiguous {dt} tensor of {n} on {dev}")
-    with _On(cached_lens) as st:
+        out = PagedLayout.empty(B, num_tokens, cached_lens.device)
+    starts, lens, slots, pos, needed = out
+    if not (starts.numel() == B + 1 and lens.numel() == B and slots.numel() == pos.numel() == num_tokens
+            and needed.numel() == 1 and slots.dtype is _I64
+            and starts.dtype is lens.dtype is pos.dtype is needed.dtype is _I32
+            and starts.get_device() == lens.get_device() == slots.get_device() == pos.get_device() == idx
+            and needed.get_device() == idx and starts.is_contiguous() and lens.is_contiguous()
+            and slots.is_contiguous() and pos.is_contiguous()):
+        raise RuntimeError(f"out must hold contiguous tensors on cuda:{idx} of PagedLayout.empty({B}, {num_tokens}, ...)'s "
+                           "sizes and types")
+    with _On(idx) as st:
         _check(_L.jo_paged_layout(cached_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(),
-                                  free_blocks.data_ptr(), B, width, stride, free_blocks.size(0), page_size, num_tokens,
-                                  out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
-                                  out[4].data_ptr(), st))
+                                  free_blocks.data_ptr(), B, width, block_tables.stride(0) if B > 1 else width,
+                                  free_blocks.numel(), page_size, num_tokens, starts.data_ptr(), lens.data_ptr(),
+                                  slots.data_ptr(), pos.data_ptr(), needed.data_ptr(), st))
     return out
 
 
-def _rows(t: torch.Tensor, name: str, dev, dtype) -> None:
-    _chk(t.is_cuda and t.device == dev, f"{name} must be a CUDA tensor on {dev}")
-    _chk(t.dtype == dtype, f"{name} dtype is {t.dtype}, expected {dtype}")
-    _chk(t.stride(-1) == 1 or t.numel() == 0, f"{name} last dim must be contiguous")
+def _refuse_layout(cached_lens, new_lens, block_tables, free_blocks, num_tokens) -> None:
+    _chk(cached_lens.is_cuda, "cached_lens must be a CUDA tensor")
+    idx = cached_lens.get_device()
+    for t, n in ((cached_lens, "cached_lens"), (new_lens, "new_lens"), (free_blocks, "free_blocks")):
+        _ints(t, n, 1, _I32, idx)
+    _ints(block_tables, "block_tables", 2, _I32, idx)       # rows may be apart: a slice of a wider table
+    B = block_tables.size(0)
+    _chk(cached_lens.numel() == B and new_lens.numel() == B,
+         "cached_lens, new_lens and block_tables must have a row per request")
+    _chk(num_tokens >= 0, "num_tokens must not be negative")
 
 
 def paged_kv_write(key, value, key_cache, value_cache, slots) -> None:
@@ -129,22 +152,37 @@ def paged_kv_write(key, value, key_cache, value_cache, slots) -> None:
     the caches [num_blocks, page_size, kv_heads, head_dim], in place.  Rows whose
     slot (int64 [T]) is negative or past the cache are left out.  Two rows must not
     have the same slot."""
-    dev, dt = key.device, key.dtype
+    idx, dt = key.get_device(), key.dtype
+    code = _DT16.get(dt)
+    T, H, D = key.shape if key.dim() == 3 else (0, 0, 0)
+    a, b, c, d = key.stride(), value.stride(), key_cache.stride(), value_cache.stride()
+    if not (idx >= 0 and code is not None and key.dim() == 3 and key.shape == value.shape and key_cache.dim() == 4
+            and value_cache.shape == key_cache.shape and key_cache.shape[2:] == key.shape[1:] and value.dtype is dt
+            and key_cache.dtype is dt and value_cache.dtype is dt and value.get_device() == idx
+            and key_cache.get_device() == idx and value_cache.get_device() == idx and a[2] == b[2] == c[3] == d[3] == 1
+            and slots.dtype is _I64 and slots.get_device() == idx and slots.dim() == 1 and slots.is_contiguous()
+            and slots.numel() == T):
+        _refuse_write(key, value, key_cache, value_cache, slots)
+    with _On(idx) as st:
+        _check(_L.jo_paged_kv_write(key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+                                    slots.data_ptr(), T, H, D, key_cache.size(0), key_cache.size(1),
+                                    _S4(a[0], a[1], b[0], b[1]), _S6(c[0], c[1], c[2], d[0], d[1], d[2]), code, st))
+
+
+def _refuse_write(key, value, key_cache, value_cache, slots) -> None:
+    _chk(key.is_cuda, "key must be a CUDA tensor")
+    idx, dt = key.get_device(), key.dtype
     _chk(dt in _DT16, "key must be bf16 or fp16")
     _chk(key.dim() == 3 and value.shape == key.shape, "key and value must be [tokens, kv_heads, head_dim]")
     _chk(key_cache.dim() == 4 and value_cache.shape == key_cache.shape and key_cache.shape[2:] == key.shape[1:],
          "caches must be [num_blocks, page_size, kv_heads, head_dim] with key's heads")
     for t, n in ((key, "key"), (value, "value"), (key_cache, "key_cache"), (value_cache, "value_cache")):
-        _rows(t, n, dev, dt)
-    _ints(slots, "slots", 1, torch.int64, dev)
-    T, H, D = key.shape
-    _chk(slots.size(0) == T, "slots must have one entry per token")
-    nb, page = key_cache.shape[:2]
-    a, b, c, d = key.stride(), value.stride(), key_cache.stride(), value_cache.stride()
-    with _On(key) as st:
-        _check(_L.jo_paged_kv_write(key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-                                    slots.data_ptr(), T, H, D, nb, page, _S2(a[0], a[1]), _S2(b[0], b[1]),
-                                    _S3(c[0], c[1], c[2]), _S3(d[0], d[1], d[2]), _DT16[dt], st))
+        _rows(t, n, dt, idx)
+    _ints(slots, "slots", 1, _I64, idx)
+    _chk(slots.numel() == key.size(0), "slots must have one entry per token")
+
+
+_ws_bytes = {}
 
 
 def varlen_attention_workspace(num_tokens: int, heads: int, head_dim: int) -> int:
@@ -155,26 +193,35 @@ def varlen_attention_workspace(num_tokens: int, heads: int, head_dim: int) -> in
     return n.value
 
 
-def _workspace(workspace, T: int, H: int, D: int, dev):
-    need = varlen_attention_workspace(T, H, D)
+def _workspace(workspace, T: int, H: int, D: int, q):
+    idx = q.get_device()
+    need = _ws_bytes.get((idx, T, H, D))
+    if need is None:
+        if len(_ws_bytes) > 4096:
+            _ws_bytes.clear()
+        with _On(idx):
+            need = _ws_bytes[(idx, T, H, D)] = varlen_attention_workspace(T, H, D)
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=dev)
-    _chk(workspace.is_cuda and workspace.device == dev and workspace.is_contiguous()
-         and workspace.numel() * workspace.element_size() >= need,
-         f"workspace must be a contiguous tensor of at least {need} bytes on {dev}")
-    return workspace
+        return torch.empty(need, dtype=torch.uint8, device=q.device), need
+    have = workspace.numel() * workspace.element_size()
+    _chk(workspace.get_device() == idx and workspace.is_contiguous() and have >= need,
+         f"workspace must be a contiguous tensor of at least {need} bytes on cuda:{idx}")
+    return workspace, have
 
 
-def _queries(q, out, dev):
-    _chk(q.is_cuda, "query must be a CUDA tensor")
-    _chk(q.dim() == 3, "query must be [tokens, heads, head_dim]")
-    _chk(q.dtype in _DT16, "query must be bf16 or fp16")
-    _rows(q, "query", dev, q.dtype)
+def _out(q, out):
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=dev)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     _chk(out.shape == q.shape, "out must have query's shape")
-    _rows(out, "out", dev, q.dtype)
+    _rows(out, "out", q.dtype, q.get_device())
     return out
+
+
+def _refuse_query(query) -> None:
+    _chk(query.is_cuda, "query must be a CUDA tensor")
+    _chk(query.dim() == 3, "query must be [tokens, heads, head_dim]")
+    _chk(query.dtype in _DT16, "query must be bf16 or fp16")
+    _rows(query, "query", query.dtype, query.get_device())
 
 
 def paged_attention(query, key_cache, value_cache, block_tables, query_starts, kv_lens, *, causal: bool = True,
@@ -194,31 +241,48 @@ def paged_attention(query, key_cache, value_cache, block_tables, query_starts, k
     kernels and never changes what is computed.  scale defaults to
     1 / sqrt(head_dim).  workspace: varlen_attention_workspace bytes, used by one
     call at a time; by default allocated per call."""
-    dev, dt = query.device, query.dtype
-    o = _queries(query, out, dev)
+    idx, dt = query.get_device(), query.dtype
+    code = _DT16.get(dt)
+    B = kv_lens.numel()
+    a, c, d = query.stride(), key_cache.stride(), value_cache.stride()
+    if not (idx >= 0 and code is not None and query.dim() == 3 and key_cache.dim() == 4
+            and value_cache.shape == key_cache.shape and a[2] == c[3] == d[3] == 1 and key_cache.size(3) == query.size(2)
+            and key_cache.dtype is dt and value_cache.dtype is dt and key_cache.get_device() == idx
+            and value_cache.get_device() == idx and block_tables.dtype is _I32 and query_starts.dtype is _I32
+            and kv_lens.dtype is _I32 and block_tables.get_device() == idx and query_starts.get_device() == idx
+            and kv_lens.get_device() == idx and block_tables.dim() == 2 and query_starts.dim() == kv_lens.dim() == 1
+            and block_tables.is_contiguous() and query_starts.is_contiguous() and kv_lens.is_contiguous()
+            and block_tables.size(0) == B and query_starts.numel() == B + 1):
+        _refuse_paged(query, key_cache, value_cache, block_tables, query_starts, kv_lens)
     T, H, D = query.shape
-    _chk(key_cache.dim() == 4 and value_cache.shape == key_cache.shape and key_cache.size(3) == D,
-         "caches must be [num_blocks, page_size, kv_heads, head_dim] with query's head_dim")
-    _rows(key_cache, "key_cache", dev, dt)
-    _rows(value_cache, "value_cache", dev, dt)
-    _ints(block_tables, "block_tables", 2, torch.int32, dev)
-    _ints(query_starts, "query_starts", 1, torch.int32, dev)
-    _ints(kv_lens, "kv_lens", 1, torch.int32, dev)
-    B, width = block_tables.shape
-    _chk(query_starts.size(0) == B + 1 and kv_lens.size(0) == B, "query_starts must have batch + 1 entries and kv_lens "
-                                                                 "batch")
+    o = _out(query, out)
     nb, page, Hk, _ = key_cache.shape
-    ws = _workspace(workspace, T, H, D, dev)
-    a, c, d, e = query.stride(), key_cache.stride(), value_cache.stride(), o.stride()
-    with _On(query) as st:
+    width = block_tables.size(1)
+    ws, ws_bytes = _workspace(workspace, T, H, D, query)
+    e = o.stride()
+    with _On(idx) as st:
         _check(_L.jo_paged_attention(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
             query_starts.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), T, B, H, Hk, D, nb, page, width,
-            block_tables.stride(0) if B > 1 else width, _S2(a[0], a[1]), _S3(c[0], c[1], c[2]), _S3(d[0], d[1], d[2]),
-            _S2(e[0], e[1]), bool(causal), 1.0 / math.sqrt(D) if scale is None else scale,
-            T if max_query_len is None else max_query_len, _DT16[dt], ws.data_ptr(),
-            ws.numel() * ws.element_size(), st))
+            block_tables.stride(0) if B > 1 else width, _S4(a[0], a[1], e[0], e[1]),
+            _S6(c[0], c[1], c[2], d[0], d[1], d[2]), bool(causal), 1.0 / math.sqrt(D) if scale is None else scale,
+            T if max_query_len is None else max_query_len, code, ws.data_ptr(), ws_bytes, st))
     return o
+
+
+def _refuse_paged(query, key_cache, value_cache, block_tables, query_starts, kv_lens) -> None:
+    _refuse_query(query)
+    idx, dt = query.get_device(), query.dtype
+    _chk(key_cache.dim() == 4 and value_cache.shape == key_cache.shape and key_cache.size(3) == query.size(2),
+         "caches must be [num_blocks, page_size, kv_heads, head_dim] with query's head_dim")
+    _rows(key_cache, "key_cache", dt, idx)
+    _rows(value_cache, "value_cache", dt, idx)
+    _ints(block_tables, "block_tables", 2, _I32, idx)       # rows may be apart: a slice of a wider table
+    _ints(query_starts, "query_starts", 1, _I32, idx)
+    _ints(kv_lens, "kv_lens", 1, _I32, idx)
+    B = block_tables.size(0)
+    _chk(query_starts.numel() == B + 1 and kv_lens.numel() == B,
+         "query_starts must have batch + 1 entries and kv_lens batch")
 
 
 def prompt_attention(query, key, value, seq_starts, *, causal: bool = True, scale: Optional[float] = None, out=None,
@@ -231,21 +295,33 @@ def prompt_attention(query, key, value, seq_starts, *, causal: bool = True, scal
     (int32 [B + 1]) of all three.  Row i sees keys 0 .. i of its own request
     (causal) or all of them.  H must be a multiple of kv_heads.  Rows of no
     request are not written.  scale, out and workspace as in paged_attention."""
-    dev, dt = query.device, query.dtype
-    o = _queries(query, out, dev)
+    idx, dt = query.get_device(), query.dtype
+    code = _DT16.get(dt)
+    a, b, c = query.stride(), key.stride(), value.stride()
+    if not (idx >= 0 and code is not None and query.dim() == 3 and key.dim() == 3 and key.shape == value.shape
+            and key.size(0) == query.size(0) and key.size(2) == query.size(2) and a[2] == b[2] == c[2] == 1
+            and key.dtype is dt and value.dtype is dt and key.get_device() == idx and value.get_device() == idx
+            and seq_starts.dtype is _I32 and seq_starts.get_device() == idx and seq_starts.dim() == 1
+            and seq_starts.is_contiguous() and seq_starts.numel() >= 1):
+        _refuse_prompt(query, key, value, seq_starts)
     T, H, D = query.shape
-    _chk(key.dim() == 3 and key.shape == value.shape and key.size(0) == T and key.size(2) == D,
-         "key and value must be [tokens, kv_heads, head_dim] with query's tokens and head_dim")
-    _rows(key, "key", dev, dt)
-    _rows(value, "value", dev, dt)
-    _ints(seq_starts, "seq_starts", 1, torch.int32, dev)
-    _chk(seq_starts.size(0) >= 1, "seq_starts must have batch + 1 entries")
-    ws = _workspace(workspace, T, H, D, dev)
-    a, b, c, e = query.stride(), key.stride(), value.stride(), o.stride()
-    with _On(query) as st:
+    o = _out(query, out)
+    ws, ws_bytes = _workspace(workspace, T, H, D, query)
+    e = o.stride()
+    with _On(idx) as st:
         _check(_L.jo_prompt_attention(
             query.data_ptr(), key.data_ptr(), value.data_ptr(), seq_starts.data_ptr(), o.data_ptr(), T,
-            seq_starts.size(0) - 1, H, key.size(1), D, _S2(a[0], a[1]), _S2(b[0], b[1]), _S2(c[0], c[1]),
-            _S2(e[0], e[1]), bool(causal), 1.0 / math.sqrt(D) if scale is None else scale, _DT16[dt], ws.data_ptr(),
-            ws.numel() * ws.element_size(), st))
+            seq_starts.numel() - 1, H, key.size(1), D, _S4(a[0], a[1], e[0], e[1]), _S4(b[0], b[1], c[0], c[1]),
+            bool(causal), 1.0 / math.sqrt(D) if scale is None else scale, code, ws.data_ptr(), ws_bytes, st))
     return o
+
+
+def _refuse_prompt(query, key, value, seq_starts) -> None:
+    _refuse_query(query)
+    idx, dt = query.get_device(), query.dtype
+    _chk(key.dim() == 3 and key.shape == value.shape and key.size(0) == query.size(0) and key.size(2) == query.size(2),
+         "key and value must be [tokens, kv_heads, head_dim] with query's tokens and head_dim")
+    _rows(key, "key", dt, idx)
+    _rows(value, "value", dt, idx)
+    _ints(seq_starts, "seq_starts", 1, _I32, idx)
+    _chk(seq_starts.numel() >= 1, "seq_starts must have batch + 1 entries")

@@ -10,7 +10,7 @@ from joyomni_ops import _lib
 
 L = _lib.lib
 BF16, F32 = _lib.JO_DTYPE_BF16, _lib.JO_DTYPE_F32
-S2, S3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+S4, S6 = ctypes.c_int64 * 4, ctypes.c_int64 * 6
 
 
 def test_wrappers_refuse_cpu_tensors():
@@ -45,8 +45,8 @@ def test_layout_refusals(kw, msg):
 
 
 def write(**kw):
-    a = dict(k=16, v=16, kc=16, vc=16, slots=16, tokens=2, heads=2, dim=64, blocks=4, page=16, ks=S2(128, 64),
-             vs=S2(128, 64), kcs=S3(2048, 128, 64), vcs=S3(2048, 128, 64), dtype=BF16)
+    a = dict(k=16, v=16, kc=16, vc=16, slots=16, tokens=2, heads=2, dim=64, blocks=4, page=16, rs=S4(128, 64, 128, 64),
+             cs=S6(2048, 128, 64, 2048, 128, 64), dtype=BF16)
     a.update(kw)
     return L.jo_paged_kv_write(*a.values(), None)
 
@@ -54,7 +54,7 @@ def write(**kw):
 @pytest.mark.parametrize("kw,code,msg", [
     (dict(dtype=F32), _lib.JO_ERR_DTYPE, "bf16 and fp16"), (dict(dim=60), _lib.JO_ERR_INVALID, "multiple of 8"),
     (dict(page=0), _lib.JO_ERR_INVALID, "invalid shape"), (dict(tokens=-1), _lib.JO_ERR_INVALID, "invalid shape"),
-    (dict(ks=S2(100, 64)), _lib.JO_ERR_ALIGN, "multiples of 8"), (dict(vcs=S3(-8, 128, 64)), _lib.JO_ERR_ALIGN, "non-negative"),
+    (dict(rs=S4(100, 64, 128, 64)), _lib.JO_ERR_ALIGN, "multiples of 8"), (dict(cs=S6(2048, 128, 64, -8, 128, 64)), _lib.JO_ERR_ALIGN, "non-negative"),
     (dict(v=24), _lib.JO_ERR_ALIGN, "16-byte"), (dict(slots=None), _lib.JO_ERR_INVALID, "null"),
 ])
 def test_write_refusals(kw, code, msg):
@@ -64,8 +64,8 @@ def test_write_refusals(kw, code, msg):
 
 def paged(**kw):
     a = dict(q=16, kc=16, vc=16, table=16, starts=16, lens=16, out=16, tokens=4, batch=2, heads=4, kv_heads=2, dim=64,
-             blocks=8, page=16, width=4, stride=4, qs=S2(256, 64), kcs=S3(2048, 128, 64), vcs=S3(2048, 128, 64),
-             os=S2(256, 64), causal=1, scale=0.1, most=4, dtype=BF16, ws=16, ws_bytes=1 << 40)
+             blocks=8, page=16, width=4, stride=4, rs=S4(256, 64, 256, 64),
+             cs=S6(2048, 128, 64, 2048, 128, 64), causal=1, scale=0.1, most=4, dtype=BF16, ws=16, ws_bytes=1 << 40)
     a.update(kw)
     return L.jo_paged_attention(*a.values(), None)
 
@@ -75,10 +75,10 @@ def paged(**kw):
     (dict(page=24), _lib.JO_ERR_INVALID, "multiple of 16"), (dict(page=0), _lib.JO_ERR_INVALID, "multiple of 16"),
     (dict(heads=5), _lib.JO_ERR_INVALID, "multiple of kv_heads"), (dict(kv_heads=0), _lib.JO_ERR_INVALID, "kv_heads"),
     (dict(heads=512), _lib.JO_ERR_INVALID, "128 times"), (dict(batch=-1), _lib.JO_ERR_INVALID, "invalid shape"),
-    (dict(width=1 << 28), _lib.JO_ERR_INVALID, "block table"), (dict(qs=S2(250, 64)), _lib.JO_ERR_ALIGN, "multiples of 8"),
-    (dict(kcs=S3(2048, -8, 64)), _lib.JO_ERR_ALIGN, "non-negative"), (dict(q=8), _lib.JO_ERR_ALIGN, "16-byte"),
+    (dict(width=1 << 28), _lib.JO_ERR_INVALID, "block table"), (dict(rs=S4(250, 64, 256, 64)), _lib.JO_ERR_ALIGN, "multiples of 8"),
+    (dict(cs=S6(2048, -8, 64, 2048, 128, 64)), _lib.JO_ERR_ALIGN, "non-negative"), (dict(q=8), _lib.JO_ERR_ALIGN, "16-byte"),
     (dict(table=None), _lib.JO_ERR_INVALID, "null"), (dict(starts=None), _lib.JO_ERR_INVALID, "null"),
-    (dict(os=None), _lib.JO_ERR_INVALID, "null strides"),
+    (dict(rs=None), _lib.JO_ERR_INVALID, "null strides"),
 ])
 def test_paged_attention_refusals(kw, code, msg):
     assert paged(**kw) == code
@@ -86,15 +86,15 @@ def test_paged_attention_refusals(kw, code, msg):
 
 
 def prompt(**kw):
-    a = dict(q=16, k=16, v=16, starts=16, out=16, tokens=4, batch=2, heads=4, kv_heads=2, dim=64, qs=S2(256, 64),
-             ks=S2(128, 64), vs=S2(128, 64), os=S2(256, 64), causal=1, scale=0.1, dtype=BF16, ws=16, ws_bytes=1 << 40)
+    a = dict(q=16, k=16, v=16, starts=16, out=16, tokens=4, batch=2, heads=4, kv_heads=2, dim=64, rs=S4(256, 64, 256, 64),
+             ks=S4(128, 64, 128, 64), causal=1, scale=0.1, dtype=BF16, ws=16, ws_bytes=1 << 40)
     a.update(kw)
     return L.jo_prompt_attention(*a.values(), None)
 
 
 @pytest.mark.parametrize("kw,code,msg", [
     (dict(dtype=F32), _lib.JO_ERR_DTYPE, "bf16 and fp16"), (dict(dim=256), _lib.JO_ERR_INVALID, "head_dim"),
-    (dict(heads=3), _lib.JO_ERR_INVALID, "multiple of kv_heads"), (dict(vs=S2(128, 60)), _lib.JO_ERR_ALIGN, "multiples of 8"),
+    (dict(heads=3), _lib.JO_ERR_INVALID, "multiple of kv_heads"), (dict(ks=S4(128, 64, 128, 60)), _lib.JO_ERR_ALIGN, "multiples of 8"),
     (dict(out=24), _lib.JO_ERR_ALIGN, "16-byte"), (dict(k=None), _lib.JO_ERR_INVALID, "null"),
     (dict(starts=None), _lib.JO_ERR_INVALID, "null"),
 ])
