@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   using C = Cfg<D>;
   constexpr int ST = C::ST;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ Steps::Scan scan;
+  __shared__ Steps::Scan<kThreads / 32> scan;
   __shared__ Steps::Near near;
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   }
   if (warp == 9) tmem_alloc_512(smem_u32(tmem_slot));
   Range range;
-  Steps::find<kThreads>(p, 2 * maps.tpt, blockIdx.x, gridDim.x, scan, near, range);
+  Steps::find<kThreads / 32>(p, 2 * maps.tpt, blockIdx.x, gridDim.x, scan, near, range);
   fence_before();
   __syncthreads();
   fence_after();

@@ -60,9 +60,16 @@ constexpr float kNoMax = -1e30f;
 
 __host__ __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
 
-constexpr int kScan = 512;               // requests of one scan of the lengths
-
 constexpr int kNear = 32;                // requests of a block's range that it keeps at hand
+
+// floor(a / b) for 0 <= a < 2^52, b > 0 (a 64-bit integer division takes some
+// hundreds of cycles, and every block's first copy waits for a few of them).
+__device__ __forceinline__ long long div_floor(long long a, long long b) {
+  long long q = (long long)((double)a / (double)b);
+  if (q * b > a) --q;
+  if ((q + 1) * b <= a) ++q;
+  return q;
+}
 
 // KEYS keys of a step.  Beginning and ending an item costs as much as LEAD steps,
 // which count as units of work too.  A cut closer than MIN steps to an item's
@@ -74,15 +81,29 @@ struct Work {
     const int last = (int)min((long long)r.n, (i + 1LL) * tpi) - 1;
     return max(1, div_up(visible(p, r, last), KEYS));
   }
-  static __device__ __forceinline__ int units(const Params& p, const Request& r, int i, int tpi) {
-    return LEAD + steps(p, r, i, tpi);
-  }
 
-  // Where a block's range of units lies.
+  // The even division of `total` units over `blocks` ranges.
+  struct Cuts {
+    long long total, each;               // the first `extra` ranges have one unit more than `each`
+    int blocks, extra;
+    __device__ __forceinline__ void divide(long long total_, int most) {
+      total = total_;
+      blocks = total >= (long long)most * (MIN + LEAD) ? most : max(1, (int)div_floor(total, MIN + LEAD));
+      each = div_floor(total, blocks);
+      extra = (int)(total - each * blocks);
+    }
+    __device__ __forceinline__ long long at(int c) const { return c >= blocks ? total : each * c + min(c, extra); }
+    // the last range that begins at or before x
+    __device__ __forceinline__ int of(long long x) const {
+      const long long big = (each + 1) * extra;
+      return x < big ? (int)div_floor(x, each + 1) : min(blocks - 1, extra + (int)div_floor(x - big, each));
+    }
+  };
+  // Where a block's range lies.
   struct Range {
     int b, h, i, step;                   // its first step, which may be its item's end
-    int blocks;                          // ranges that are not empty by intent
-    long long begin, end, total;
+    long long begin, end;                // units
+    Cuts cuts;
   };
   // The range's requests, as far as they have room: every role of the block
   // walks over them, and a look at the lengths in global memory for each would
@@ -92,132 +113,145 @@ struct Work {
     int b[kNear];
     Request r[kNear];
   };
-  static __device__ __forceinline__ long long cut_at(long long total, int blocks, int c) {
-    return c >= blocks ? total : total / blocks * c + total % blocks * c / blocks;
-  }
-
-  struct Scan {
-    int first[kScan], n[kScan], keys[kScan];
-    long long before[kScan + 1];         // units before each request of the scan
-    Range cut[2];
-    long long at[2];
+  struct Place {                         // a cut: the request it falls into and the units before it there
+    int b, rank;
+    long long off, per_head, at;
+    Request r;
+    int h, i, step;
+  };
+  template <int WARPS> struct Scan {
+    longlong2 sums[WARPS];               // units, requests with rows
+    Place cut[2];
   };
 
-  // Range of block c of at most C.  All THREADS threads of the block take part.
-  template <int THREADS>
-  static __device__ void find(const Params& p, int tpi, int c, int C, Scan& s, Near& near, Range& range) {
+  // Units of one key head of a request, by one thread or by a warp.
+  static __device__ __forceinline__ long long head_units(const Params& p, const Request& r, int tpi, int from, int by) {
+    const int ni = div_up(r.n, tpi);
+    long long u = 0;
+    for (int q = from; q < ni; q += by) u += LEAD + steps(p, r, q, tpi);
+    return u;
+  }
+
+  // Range of block c of at most C.  All threads of the block (WARPS warps) take
+  // part, each looking after one request of a run of as many as there are threads.
+  // Latency-bound: one look at the lengths, a scan over the block, two divisions.
+  template <int WARPS>
+  static __device__ void find(const Params& p, int tpi, int c, int C, Scan<WARPS>& s, Near& near, Range& range) {
+    constexpr int THREADS = 32 * WARPS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int chunks = div_up(p.batch, kScan);
-    long long total = 0, target = 0;
-    int blocks = C;
-    // First time round: the number of units.  Second: the places of the cuts.
-    for (int round = 0; round < 2; ++round) {
-      if (round == 1) {
-        blocks = (int)max(1LL, min((long long)C, total / (MIN + LEAD)));
-        target = warp < 2 ? cut_at(total, blocks, c + warp) : total;
-        if (warp < 2 && lane == 0) {
-          s.cut[warp] = Range{p.batch, 0, 0, 0, 0, 0, 0, 0};
-          s.at[warp] = total;
+    const bool one = p.batch <= THREADS; // one run holds them all
+    Cuts cuts;
+    long long begin = 0, end = 0;
+    // First time round: the number of units, and where one run holds all the
+    // cuts too.  Second: the cuts.
+    for (int round = one ? 1 : 0; round < 2; ++round) {
+      longlong2 base = make_longlong2(0, 0);
+      for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
+        const int b = b0 + threadIdx.x;
+        Request r{0, 0, 0};
+        if (b < p.batch) r = request(p, b);
+        long long u = 0;
+        const bool many = r.n > 16 * tpi; // too many items for one thread
+        if (!many) u = head_units(p, r, tpi, 0, 1);
+        for (unsigned left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
+          const int src = __ffs(left) - 1;
+          const Request w{0, __shfl_sync(0xffffffffu, r.n, src), __shfl_sync(0xffffffffu, r.keys, src)};
+          long long v = head_units(p, w, tpi, lane, 32);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          if (lane == src) u = v;
         }
-        __syncwarp();
+        const longlong2 mine = make_longlong2(u * p.kv_heads, r.n > 0);
+        longlong2 before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long x = __shfl_up_sync(0xffffffffu, before.x, o), y = __shfl_up_sync(0xffffffffu, before.y, o);
+          if (lane >= o) before.x += x, before.y += y;
+        }
+        __syncthreads();                 // the run before has been read
+        if (lane == 31) s.sums[warp] = before;
+        __syncthreads();
+        before.x += base.x - mine.x;
+        before.y += base.y - mine.y;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const longlong2 x = s.sums[w];
+          if (w < warp) before.x += x.x, before.y += x.y;
+          base.x += x.x, base.y += x.y;
+        }
+        if (round == 0) continue;
+        if (one) {
+          cuts.divide(base.x, C);
+          begin = cuts.at(c);
+          end = cuts.at(c + 1);
+        }
+        if (b0 == 0) {
+          if (threadIdx.x < 2) s.cut[threadIdx.x] = Place{p.batch, 0, 0, 1, end, {0, 0, 0}, 0, 0, 0};
+          __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const long long t = k ? end : begin;
+          if (t >= before.x && t < before.x + mine.x)
+            s.cut[k] = Place{b, (int)before.y, t - before.x, u, t, r, 0, 0, 0};
+        }
+        if (one) {                       // this thread's request may be one of the range's
+          __syncthreads();
+          const int at = (int)before.y - s.cut[0].rank;
+          if (r.n > 0 && b >= s.cut[0].b && b <= s.cut[1].b && at < kNear) {
+            near.b[at] = b;
+            near.r[at] = r;
+          }
+        }
       }
-      long long base = 0;
-      for (int ch = 0; ch < chunks; ++ch) {
-        const int cnt = min(kScan, p.batch - ch * kScan);
-        if (round == 0 || chunks > 1) {
-          __syncthreads();
-          for (int i = threadIdx.x; i < cnt; i += THREADS) {
-            const Request r = request(p, ch * kScan + i);
-            s.first[i] = r.first;
-            s.n[i] = r.n;
-            s.keys[i] = r.keys;
-          }
-          __syncthreads();
-          for (int i = warp; i < cnt; i += THREADS / 32) {
-            const Request r{s.first[i], s.n[i], s.keys[i]};
-            const int ni = div_up(r.n, tpi);
-            long long u = 0;
-            for (int q = lane; q < ni; q += 32) u += units(p, r, q, tpi);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-            if (lane == 0) s.before[i + 1] = u * p.kv_heads;
-          }
-          __syncthreads();
-          if (warp == 0) {
-            constexpr int E = kScan / 32;
-            long long mine = 0;
-            for (int i = lane * E; i < min(cnt, lane * E + E); ++i) mine += s.before[i + 1];
-            long long inc = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-              if (lane >= o) inc += x;
-            }
-            long long run = inc - mine;
-            if (lane == 0) s.before[0] = 0;
-            for (int i = lane * E; i < min(cnt, lane * E + E); ++i) {
-              run += s.before[i + 1];
-              s.before[i + 1] = run;
-            }
-          }
-          __syncthreads();
-        }
-        const long long sum = s.before[cnt];
-        if (round == 1 && warp < 2 && target >= base && target < base + sum) {
-          const long long rel = target - base;
-          int a = 0, e = cnt;            // last request that begins at or before rel
-          while (e - a > 1) {
-            const int mid = (a + e) >> 1;
-            if (s.before[mid] <= rel) a = mid; else e = mid;
-          }
-          const Request r{s.first[a], s.n[a], s.keys[a]};
-          const long long per_head = (s.before[a + 1] - s.before[a]) / p.kv_heads;
-          const long long in_req = rel - s.before[a];
-          const int h = (int)(in_req / per_head);
-          long long off = in_req - h * per_head;
-          const int ni = div_up(r.n, tpi);
-          for (int q0 = 0; q0 < ni; q0 += 32) {
-            const int q = q0 + lane;
-            const long long u = q < ni ? units(p, r, q, tpi) : 0;
-            long long inc = u;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-              if (lane >= o) inc += x;
-            }
-            const unsigned hit = __ballot_sync(0xffffffffu, inc > off);
-            if (hit) {
-              if (lane == __ffs(hit) - 1) {
-                long long step = off - (inc - u) - LEAD, at = target;
-                const long long last = u - LEAD;
-                if (step < MIN) {
-                  at -= step + LEAD;
-                  step = 0;
-                } else if (last - step < MIN) {
-                  at += last - step;
-                  step = last;
-                }
-                s.cut[warp] = Range{ch * kScan + a, h, q, (int)step, 0, 0, 0, 0};
-                s.at[warp] = at;
-              }
-              break;
-            }
-            off -= __shfl_sync(0xffffffffu, inc, 31);
-          }
-        }
-        base += sum;
+      if (round == 0) {
+        cuts.divide(base.x, C);
+        begin = cuts.at(c);
+        end = cuts.at(c + 1);
+      } else if (one && threadIdx.x == 0) {
+        const int first = s.cut[0].b < p.batch ? s.cut[0].rank : (int)base.y;
+        const int last = s.cut[1].b < p.batch ? s.cut[1].rank + 1 : (int)base.y;
+        near.count = min(kNear, max(0, last - first));
       }
-      total = base;
     }
     __syncthreads();
-    range = s.cut[0];
-    range.blocks = blocks;
-    range.begin = s.at[0];
-    range.end = s.at[1];
-    range.total = total;
-    const int last = min(s.cut[1].b, p.batch - 1);
-    if (warp == 0) {
-      int count = 0, b0 = range.b;
+    // head, item and step of the two cuts, a warp for each
+    if (warp < 2 && s.cut[warp].b < p.batch) {
+      Place& f = s.cut[warp];
+      const int h = (int)div_floor(f.off, f.per_head), ni = div_up(f.r.n, tpi);
+      long long off = f.off - h * f.per_head;
+      for (int q0 = 0; q0 < ni; q0 += 32) {
+        const int q = q0 + lane, n = q < ni ? steps(p, f.r, q, tpi) : 0;
+        long long inc = q < ni ? LEAD + n : 0;
+        const long long u = inc;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += x;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, inc > off);
+        if (hit) {
+          if (lane == __ffs(hit) - 1) {
+            long long step = off - (inc - u) - LEAD;
+            if (step < MIN) {
+              f.at -= step + LEAD;
+              step = 0;
+            } else if (n - step < MIN) {
+              f.at += n - step;
+              step = n;
+            }
+            f.h = h;
+            f.i = q;
+            f.step = (int)step;
+          }
+          break;
+        }
+        off -= __shfl_sync(0xffffffffu, inc, 31);
+      }
+    }
+    if (!one && warp == 2) {             // the range's requests, looked up again
+      const int last = min(s.cut[1].b, p.batch - 1);
+      int count = 0, b0 = s.cut[0].b;
       for (; b0 <= last && count < kNear; b0 += 32) {
         Request r{0, 0, 0};
         if (b0 + lane <= last) r = request(p, b0 + lane);
@@ -229,12 +263,11 @@ struct Work {
         }
         count += __popc(any);
       }
-      __syncwarp();
-      if (lane == 0) {
-        near.count = min(count, kNear);
-        near.next = count > kNear ? near.b[kNear - 1] + 1 : b0;
-      }
+      if (lane == 0) near.count = min(count, kNear);
     }
+    __syncthreads();
+    if (threadIdx.x == 0) near.next = near.count > 0 ? near.b[near.count - 1] + 1 : p.batch;
+    range = Range{s.cut[0].b, s.cut[0].h, s.cut[0].i, s.cut[0].step, s.cut[0].at, s.cut[1].at, cuts};
   }
 
   // One block's stretch of one item.
@@ -306,14 +339,11 @@ struct Work {
     }
   };
 
-  // Blocks after this one that have a piece of the item that piece s begins.
+  // Blocks after this one that have a piece of the item that piece s begins: the
+  // last of them begins before the item's end, and not so close to it that its
+  // cut moved there.
   static __device__ int later_blocks(const Range& g, const Piece& s, int c) {
-    // block c' has one if its cut is not past the item's end, nor so close to it that it moved there
-    const long long x = s.at + s.steps - MIN;
-    int last = (int)min((long long)g.blocks - 1, (x + 1) * g.blocks / g.total);
-    while (last + 1 < g.blocks && cut_at(g.total, g.blocks, last + 1) <= x) ++last;
-    while (last > c && cut_at(g.total, g.blocks, last) > x) --last;
-    return last - c;
+    return g.cuts.of(s.at + s.steps - MIN) - c;
   }
 };
 

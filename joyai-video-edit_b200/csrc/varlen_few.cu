@@ -5,11 +5,11 @@
 // worth of arithmetic.  So the organisation is the one that keeps the most bytes
 // in flight with the least work per byte: two blocks on every SM, each with 96 KB
 // of K and V steps (64 keys) on the way through TMA, looked after by one warp,
-// and four warps that take 16 keys of a step each with mma.sync (m16n8k16: its 16
-// rows fit a group, where the 128 of a tcgen05 tile would be mostly empty).  The
-// four warps keep maxima, sums and accumulators of their own and meet only at the
-// end of an item's piece, not at every step.  The steps of all items are shared
-// out evenly over the blocks (varlen_attention.cuh).
+// and four warps on mma.sync (m16n8k16: its 16 rows fit a group, where the 128 of
+// a tcgen05 tile would be mostly empty).  Of a step's scores each warp has 16
+// keys, of its output a quarter of the columns; the weights change hands in
+// shared memory, with one barrier a step.  The steps of all items are shared out
+// evenly over the blocks (varlen_attention.cuh).
 #include "varlen_attention.cuh"
 
 namespace jo {
@@ -35,17 +35,15 @@ template <int D, int MT> struct Cfg {
   static constexpr int HALVES = D / 64, HALF = kKeys * 128;  // 64 columns: 128-byte rows
   static constexpr int TILE = HALVES * HALF;                 // K or V of a step
   static constexpr int ST = D == 128 ? 3 : 6;                // steps in flight: 96 KB
-  // During the steps: Q, then weights of the careful product.  After them: the
-  // warps' maxima and sums, then the R x D result in fp32.
-  static constexpr int MERGE = ST * 2 * TILE;
-  static constexpr int WEIGHTS = R * D * 2;
-  static constexpr int SPACE = WEIGHTS + kWarps * R * 64 > R * D * 4 ? WEIGHTS + kWarps * R * 64 : R * D * 4;
-  static constexpr int BARS = MERGE + SPACE;
+  static constexpr int Q0 = ST * 2 * TILE;                   // Q: R rows, 16-byte pieces turned as the swizzle does
+  static constexpr int P0 = Q0 + R * D * 2;                  // weights: two buffers of R rows of 64 keys, likewise
+  static constexpr int P_BYTES = R * kKeys * 2;
+  static constexpr int BARS = P0 + 2 * P_BYTES;
   static constexpr int NEAR = BARS + 128;
   static constexpr int BYTES = NEAR + (int)sizeof(Steps::Near);
   static_assert(2 * ST * 8 + 4 <= 128, "");
+  static_assert(kWarps * R * 4 <= P_BYTES, "");
   static_assert(BYTES + 1024 <= 228 * 1024 / kBlocksPerSm, "");
-  static_assert(sizeof(Steps::Scan) <= (size_t)MERGE, "");
 };
 
 struct Maps {
@@ -79,8 +77,18 @@ template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], cons
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The barrier of the computing warps.
+// The barrier of the computing warps, and the one that tells whether any thread's flag is set.
 __device__ __forceinline__ void team_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+
+__device__ __forceinline__ bool team_any(bool flag) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, 1, %2, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)flag), "n"(32 * kWarps)
+      : "memory");
+  return r != 0;
+}
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __grid_constant__ Maps maps, const Params p) {
@@ -89,7 +97,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * ST);
-  float* merge = reinterpret_cast<float*>(smem + C::MERGE);
   Steps::Near& near = *reinterpret_cast<Steps::Near*>(smem + C::NEAR);
   const uint32_t bar0 = smem_u32(bars), ring = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -98,6 +105,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
 
   launch_dependents();
   if (threadIdx.x == 0) {
+    tma_prefetch_map(&maps.k);
+    tma_prefetch_map(&maps.v);
     for (int s = 0; s < ST; ++s) {
       mbar_init(FULL(s), 1);
       mbar_init(EMPTY(s), kWarps);
@@ -109,7 +118,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   Range range;
-  Steps::find<kThreads>(p, maps.tpi, blockIdx.x, gridDim.x, *reinterpret_cast<Steps::Scan*>(smem), near, range);
+  using Scan = Steps::Scan<kThreads / 32>;
+  Steps::find<kThreads / 32>(p, maps.tpi, blockIdx.x, gridDim.x, *reinterpret_cast<Scan*>(smem), near, range);
   fence_async_smem();                    // the scan's space becomes the ring
   __syncthreads();
   const int tpi = maps.tpi;
@@ -150,20 +160,21 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
     }
   } else {
     // -------------------------------------------------------------- compute --
+    constexpr int NW = D / 8 / kWarps;                       // 8-column blocks of this warp's output
     const int qr = lane >> 2, qc = (lane & 3) * 2;           // row and columns of this lane in a fragment
     const float c = p.scale_log2;
     // ldmatrix: row and 8-column block that this lane points at
     const int krow = warp * 16 + (lane >> 4) * 8 + (lane & 7), kcol = (lane >> 3) & 1;
-    const int vrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), vcol = lane >> 4;
-    const int qrow = lane & 15, qcol = lane >> 4;
-    const uint32_t qs = ring + C::MERGE;
+    const int vrow = ((lane >> 3) & 1) * 8 + (lane & 7), vcol = lane >> 4;
+    const int arow = lane & 15, acol = lane >> 4;
+    const uint32_t qs = ring + C::Q0, ps = ring + C::P0;
     uint32_t it = 0;
-    // After a wait that gave up the warps skip the steps but still walk the pieces:
-    // they meet at the barriers below, which have no limit.
+    // After a wait that gave up the warps skip the steps but still walk the pieces
+    // (and every one of them skips the same ones): they meet at barriers, which
+    // have no limit.
     while (walk.next(s)) {
       const int tok0 = s.i * tpi, ntok = min(tpi, s.r.n - tok0);
       const int some = visible(p, s.r, tok0), most = visible(p, s.r, tok0 + ntok - 1);
-      // Q, in 16-byte pieces turned by the row as the swizzle does
       for (int i = threadIdx.x; i < R * (D / 8); i += 32 * kWarps) {
         const int r = i / (D / 8), n = i % (D / 8), tok = r / p.group, g = r - tok * p.group;
         uint4 x = make_uint4(0, 0, 0, 0);
@@ -172,31 +183,29 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
                                               (int64_t)(s.h * p.group + g) * p.q_hs + n * 8);
           if (p.negate) x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
         }
-        *reinterpret_cast<uint4*>(smem + C::MERGE + r * D * 2 + ((n ^ (r & 7)) << 4)) = x;
+        *reinterpret_cast<uint4*>(smem + C::Q0 + r * D * 2 + ((n ^ (r & 7)) << 4)) = x;
       }
       int limit[MT][2];                                      // keys that this lane's rows see
+      float o[MT][NW][4], m[MT][2], l[MT][2];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int tok = (t * 16 + e * 8 + qr) / p.group;
           limit[t][e] = tok < ntok ? visible(p, s.r, tok0 + tok) : 0;
+          m[t][e] = kNoMax;
+          l[t][e] = 0.f;
         }
-      float o[MT][D / 8][4], m[MT][2], l[MT][2];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        m[t][0] = m[t][1] = kNoMax;
-        l[t][0] = l[t][1] = 0.f;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
+        for (int n = 0; n < NW; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
       }
       team_sync();
-      for (int j = s.a; j < s.e && ok; ++j, ++it) {
+      for (int j = s.a; j < s.e; ++j, ++it) {
         const int st = it % ST;
-        ok = __all_sync(0xffffffffu, mbar_wait(FULL(st), (it / ST) & 1, abort_flag, &g_fault, 102));
-        if (!ok) break;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(FULL(st), (it / ST) & 1, abort_flag, &g_fault, 102));
         const uint32_t ks = ring + st * 2 * C::TILE, vs = ks + C::TILE;
         const int key0 = j * kKeys + warp * 16;              // this warp's keys
+        const uint32_t pbuf = ps + (it & 1) * C::P_BYTES;
         float x[MT][2][4];
 #pragma unroll
         for (int t = 0; t < MT; ++t)
@@ -209,13 +218,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
             uint32_t a[4];
-            ldsm4(qs + (t * 16 + qrow) * D * 2 + (((k * 2 + qcol) ^ (qrow & 7)) << 4), a);
+            ldsm4(qs + (t * 16 + arow) * D * 2 + (((k * 2 + acol) ^ (arow & 7)) << 4), a);
             mma16816<T>(x[t][0], a, b[0], b[1]);
             mma16816<T>(x[t][1], a, b[2], b[3]);
           }
         }
+        const bool edge = (j + 1) * kKeys > some;            // some row does not see every key of this step
         int bad = 0;
-        if (key0 + 16 > some) {                              // some row does not see every key
+        if (edge) {
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -223,14 +233,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 if (key0 + n * 8 + qc + (i & 1) >= limit[t][i >> 1]) x[t][n][i] = -INFINITY;
-          // a product with a weight of 0 would turn a NaN in V into NaN: rows
-          // that no query row sees are zeroed, others are searched
+          // a product with a weight of 0 would turn a NaN in V into NaN: in this
+          // warp's columns, keys that no row sees are zeroed, others are searched
           unsigned char* v = smem + st * 2 * C::TILE + C::TILE;
-          constexpr int CH = D / 8;
-          for (int i = max(0, some - key0) * CH + lane; i < 16 * CH; i += 32) {
-            const int row = i / CH;
-            uint4* y = reinterpret_cast<uint4*>(v + swizzled(warp * 16 + row, (i % CH) * 8, C::HALF));
-            if (key0 + row >= most) {
+          for (int i = max(0, some - j * kKeys) * NW + lane; i < kKeys * NW; i += 32) {
+            const int row = i / NW;
+            uint4* y = reinterpret_cast<uint4*>(v + swizzled(row, (warp * NW + i % NW) * 8, C::HALF));
+            if (j * kKeys + row >= most) {
               *y = make_uint4(0, 0, 0, 0);
             } else {
               constexpr uint32_t EL = Bits16<T>::kInf, EH = EL << 16;
@@ -242,85 +251,109 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
           fence_async_smem();                                // the next copy into this place comes after these writes
           bad = __any_sync(0xffffffffu, bad);
         }
+        // The maximum only moves when it grows by more than 2^8 somewhere: the
+        // weights are made with the old one, and again in the rare other case.
+        float top[MT][2];
         bool raise = false;
-        float alpha[MT][2];
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float mx = fmaxf(fmaxf(x[t][0][2 * e], x[t][0][2 * e + 1]), fmaxf(x[t][1][2 * e], x[t][1][2 * e + 1]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * c;
-            // the maximum only moves when it grows by more than 2^8
-            const bool need = mx > m[t][e] + 8.f;
-            const float mn = need ? mx : m[t][e];
-            alpha[t][e] = ex2(m[t][e] - mn);
-            raise |= need;
-            m[t][e] = mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int i = 2 * e; i < 2 * e + 2; ++i) {
-                x[t][n][i] = ex2(fmaf(x[t][n][i], c, -mn));
-                sum += x[t][n][i];
-              }
-            l[t][e] = fmaf(l[t][e], alpha[t][e], sum);
+            top[t][e] = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * c;
+            raise |= top[t][e] > m[t][e] + 8.f;
           }
-        if (__any_sync(0xffffffffu, raise)) {
+        float sum[MT][2];
+        auto weigh = [&]() {
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n)
+            for (int e = 0; e < 2; ++e) {
+              const int r = t * 16 + e * 8 + qr;
+              sum[t][e] = 0.f;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o[t][n][i] *= alpha[t][i >> 1];
+              for (int n = 0; n < 2; ++n) {
+                const float a = ex2(fmaf(x[t][n][2 * e], c, -m[t][e])), b = ex2(fmaf(x[t][n][2 * e + 1], c, -m[t][e]));
+                sum[t][e] += a + b;
+                // rounded to the tensors' type for the product with V; the sum is of the unrounded ones
+                *reinterpret_cast<uint32_t*>(smem + (pbuf - ring) + r * 128 + (((warp * 2 + n) ^ (r & 7)) << 4) + qc * 2) =
+                    pack2<T>(a, b);
+              }
+            }
+        };
+        weigh();
+        if (team_any(raise)) {
+          // all are past the step before, so its buffer has room for the maxima
+          float* tops = reinterpret_cast<float*>(smem + C::P0 + ((it + 1) & 1) * C::P_BYTES);
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if ((lane & 3) == 0) tops[warp * R + t * 16 + e * 8 + qr] = top[t][e];
+          team_sync();
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = kNoMax;
+#pragma unroll
+              for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, tops[w * R + t * 16 + e * 8 + qr]);
+              const float mn = mx > m[t][e] + 8.f ? mx : m[t][e], alpha = ex2(m[t][e] - mn);
+              m[t][e] = mn;
+              l[t][e] *= alpha;
+#pragma unroll
+              for (int n = 0; n < NW; ++n) {
+                o[t][n][2 * e] *= alpha;
+                o[t][n][2 * e + 1] *= alpha;
+              }
+            }
+          weigh();
+          team_sync();
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          l[t][0] += sum[t][0];
+          l[t][1] += sum[t][1];
         }
         if (!bad) {
-          // the weights are rounded to the tensors' type for the product with V;
-          // their sum is of the unrounded ones
-          uint32_t a[MT][4];
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            a[t][0] = pack2<T>(x[t][0][0], x[t][0][1]);
-            a[t][1] = pack2<T>(x[t][0][2], x[t][0][3]);
-            a[t][2] = pack2<T>(x[t][1][0], x[t][1][1]);
-            a[t][3] = pack2<T>(x[t][1][2], x[t][1][3]);
-          }
+          for (int k = 0; k < kKeys / 16; ++k) {
+            uint32_t a[MT][4];
 #pragma unroll
-          for (int n = 0; n < D / 16; ++n) {
-            uint32_t b[4];
-            ldsm4_t(vs + (n >> 2) * C::HALF + vrow * 128 + ((((n & 3) * 2 + vcol) ^ (vrow & 7)) << 4), b);
+            for (int t = 0; t < MT; ++t)
+              ldsm4(pbuf + (t * 16 + arow) * 128 + (((k * 2 + acol) ^ (arow & 7)) << 4), a[t]);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              mma16816<T>(o[t][2 * n], a[t], b[0], b[1]);
-              mma16816<T>(o[t][2 * n + 1], a[t], b[2], b[3]);
+            for (int n = 0; n < NW / 2; ++n) {
+              const int col = warp * NW + 2 * n + vcol;      // 8-column block
+              uint32_t b[4];
+              ldsm4_t(vs + (col >> 3) * C::HALF + (k * 16 + vrow) * 128 + (((col & 7) ^ (vrow & 7)) << 4), b);
+#pragma unroll
+              for (int t = 0; t < MT; ++t) {
+                mma16816<T>(o[t][2 * n], a[t], b[0], b[1]);
+                mma16816<T>(o[t][2 * n + 1], a[t], b[2], b[3]);
+              }
             }
           }
         } else {
           // a NaN or infinity that only some rows may see: row by row on the CUDA cores
-          float* w = reinterpret_cast<float*>(smem + C::MERGE + C::WEIGHTS) + warp * R * 16;
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[(t * 16 + (i >> 1) * 8 + qr) * 16 + n * 8 + qc + (i & 1)] = x[t][n][i];
-          __syncwarp();
           const unsigned char* v = smem + st * 2 * C::TILE + C::TILE;
 #pragma unroll 1
-          for (int k = 0; k < 16; ++k) {
+          for (int k = 0; k < kKeys; ++k) {
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
+            for (int n = 0; n < NW; ++n) {
               const float2 f =
-                  unpack2<T>(*reinterpret_cast<const uint32_t*>(v + swizzled(warp * 16 + k, n * 8 + qc, C::HALF)));
+                  unpack2<T>(*reinterpret_cast<const uint32_t*>(v + swizzled(k, (warp * NW + n) * 8 + qc, C::HALF)));
 #pragma unroll
               for (int t = 0; t < MT; ++t)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                  if (key0 + k < limit[t][e]) {
-                    const float pw = w[(t * 16 + e * 8 + qr) * 16 + k];
-                    o[t][n][2 * e] = fmaf(pw, f.x, o[t][n][2 * e]);
-                    o[t][n][2 * e + 1] = fmaf(pw, f.y, o[t][n][2 * e + 1]);
+                  if (j * kKeys + k < limit[t][e]) {
+                    const int r = t * 16 + e * 8 + qr;
+                    const float w = to_f32(*reinterpret_cast<const T*>(smem + (pbuf - ring) + r * 128 +
+                                                                       (((k >> 3) ^ (r & 7)) << 4) + (k & 7) * 2));
+                    o[t][n][2 * e] = fmaf(w, f.x, o[t][n][2 * e]);
+                    o[t][n][2 * e + 1] = fmaf(w, f.y, o[t][n][2 * e + 1]);
                   }
             }
           }
@@ -328,73 +361,45 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
         __syncwarp();
         if (lane == 0) mbar_arrive(EMPTY(st));
       }
-      // ---- the four warps' results together, in their order ----
-      team_sync();                                           // the space has been read as Q
+      // ---- the rows' sums over the four warps, then the result ----
+      team_sync();                                           // the weights have been read
+      float* sums = reinterpret_cast<float*>(smem + C::P0);
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 1);
           l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 2);
-          if ((lane & 3) == 0) reinterpret_cast<float2*>(merge)[warp * R + t * 16 + e * 8 + qr] = make_float2(m[t][e], l[t][e]);
+          if ((lane & 3) == 0) sums[warp * R + t * 16 + e * 8 + qr] = l[t][e];
         }
       team_sync();
       const bool whole = s.whole();
       Slot<D, 32>& slot = static_cast<Slot<D, 32>*>(maps.partial)[2 * blockIdx.x + (s.a == 0 ? 1 : 0)];
-      float f[MT][2];                                        // this warp's factor of each row
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = t * 16 + e * 8 + qr;
-          float top = kNoMax, sum = 0.f;
+          const int r = t * 16 + e * 8 + qr, tok = r / p.group, g = r - tok * p.group;
+          float sum = 0.f;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, reinterpret_cast<float2*>(merge)[w * R + r].x);
+          for (int w = 0; w < kWarps; ++w) sum += sums[w * R + r];
+          if (tok >= ntok) continue;
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* row = static_cast<T*>(p.out) + (int64_t)(s.r.first + tok0 + tok) * p.o_ts + (int64_t)(s.h * p.group + g) * p.o_hs +
+                     warp * NW * 8 + qc;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float2 ml = reinterpret_cast<float2*>(merge)[w * R + r];
-            sum = fmaf(ml.y, ex2(ml.x - top), sum);
-          }
-          f[t][e] = ex2(m[t][e] - top);
-          if (whole) f[t][e] *= sum == 0.f ? 0.f : 1.f / sum;
-          else if (warp == 0 && (lane & 3) == 0) slot.ml[r] = make_float2(top, sum);
-        }
-      team_sync();
-      // R x D, the 8-column blocks of row r turned by r so that a fragment's rows meet different banks
-#pragma unroll 1
-      for (int w = 0; w < kWarps; ++w) {
-        if (warp == w) {
+            for (int n = 0; n < NW; ++n)
+              *reinterpret_cast<uint32_t*>(row + n * 8) = pack2<T>(o[t][n][2 * e] * inv, o[t][n][2 * e + 1] * inv);
+          } else {
+            if (warp == 0 && (lane & 3) == 0) slot.ml[r] = make_float2(m[t][e], sum);
 #pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = t * 16 + e * 8 + qr;
-#pragma unroll
-              for (int n = 0; n < D / 8; ++n) {
-                float2* at = reinterpret_cast<float2*>(merge + r * D + ((n + r) % (D / 8)) * 8 + qc);
-                const float2 was = w ? *at : make_float2(0.f, 0.f);
-                *at = make_float2(fmaf(o[t][n][2 * e], f[t][e], was.x), fmaf(o[t][n][2 * e + 1], f[t][e], was.y));
-              }
+            for (int n = 0; n < NW; ++n) {
+              const int col = (warp * NW + n) * 8 + qc;
+              *reinterpret_cast<float2*>(&slot.o[col / 4][r][col % 4]) = make_float2(o[t][n][2 * e], o[t][n][2 * e + 1]);
             }
+          }
         }
-        team_sync();
-      }
-      for (int i = threadIdx.x; i < R * (D / 8); i += 32 * kWarps) {
-        const int r = whole ? i / (D / 8) : i % R, n = whole ? i % (D / 8) : i / R;
-        const int tok = r / p.group, g = r - tok * p.group;
-        if (tok >= ntok) continue;
-        const float4* at = reinterpret_cast<const float4*>(merge + r * D + ((n + r) % (D / 8)) * 8);
-        const float4 a = at[0], b = at[1];
-        if (whole) {
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)(s.r.first + tok0 + tok) * p.o_ts +
-                                    (int64_t)(s.h * p.group + g) * p.o_hs + n * 8) =
-              make_uint4(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w), pack2<T>(b.x, b.y), pack2<T>(b.z, b.w));
-        } else {
-          *reinterpret_cast<float4*>(slot.o[2 * n][r]) = a;
-          *reinterpret_cast<float4*>(slot.o[2 * n + 1][r]) = b;
-        }
-      }
-      team_sync();
     }
   }
 #undef FULL
