@@ -163,18 +163,32 @@ struct WriteParams {
   int64_t k_ts, k_hs, v_ts, v_hs, kc_bs, kc_ts, kc_hs, vc_bs, vc_ts, vc_hs;
 };
 
-// One thread per 16-byte vector of a token's K and V rows.
+// A thread takes the same 16-byte vector of K and of V of kTokens tokens, all loads before the first store: bound by HBM, and four
+// loads in flight per thread keep it busy (one token a thread: 21.3 us for 11042
+// tokens of 10 heads of 128, 5.3 TB/s).
+constexpr int kTokens = 2;
 __global__ void __launch_bounds__(kThreads) write_kernel(const WriteParams p) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t t = i / p.row_vecs;
-  if (t >= p.tokens) return;
-  const int64_t slot = p.slots[t];
-  if (slot < 0 || slot >= p.num_slots) return;
-  const uint32_t x = (uint32_t)(i - t * p.row_vecs);
+  const uint32_t x = blockIdx.y * blockDim.x + threadIdx.x;
+  if (x >= p.row_vecs) return;
   const uint32_t h = x / p.head_vecs, d = x - h * p.head_vecs;
-  const int64_t block = slot / p.page, in_page = slot - block * p.page;
-  p.kc[block * p.kc_bs + in_page * p.kc_ts + h * p.kc_hs + d] = ld_stream(p.k + t * p.k_ts + h * p.k_hs + d);
-  p.vc[block * p.vc_bs + in_page * p.vc_ts + h * p.vc_hs + d] = ld_stream(p.v + t * p.v_ts + h * p.v_hs + d);
+  const int64_t t0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * kTokens;
+  int64_t slot[kTokens];
+  uint4 k[kTokens], v[kTokens];
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) slot[i] = t0 + i < p.tokens ? p.slots[t0 + i] : -1;
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i)
+    if (t0 + i < p.tokens) {
+      k[i] = ld_stream(p.k + (t0 + i) * p.k_ts + h * p.k_hs + d);
+      v[i] = ld_stream(p.v + (t0 + i) * p.v_ts + h * p.v_hs + d);
+    }
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i)
+    if (slot[i] >= 0 && slot[i] < p.num_slots) {
+      const int64_t block = slot[i] / p.page, in_page = slot[i] - block * p.page;
+      p.kc[block * p.kc_bs + in_page * p.kc_ts + h * p.kc_hs + d] = k[i];
+      p.vc[block * p.vc_bs + in_page * p.vc_ts + h * p.vc_hs + d] = v[i];
+    }
 }
 
 }  // namespace paged
@@ -249,9 +263,14 @@ int jo_paged_kv_write(const void* key, const void* value, void* key_cache, void*
   p.row_vecs = (uint32_t)(kv_heads * (head_dim / 8));
   int64_t* dst[10] = {&p.k_ts, &p.k_hs, &p.v_ts, &p.v_hs, &p.kc_bs, &p.kc_ts, &p.kc_hs, &p.vc_bs, &p.vc_ts, &p.vc_hs};
   for (int i = 0; i < 10; ++i) *dst[i] = all[i] / 8;
-  const int64_t blocks = (tokens * p.row_vecs + paged::kThreads - 1) / paged::kThreads;
-  JO_REQUIRE(blocks < (1LL << 31), JO_ERR_INVALID, "paged_kv_write: too many elements");
-  paged::write_kernel<<<(unsigned)blocks, paged::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  // as many threads along a token's vectors as it has, up to a block's, and the rest along tokens
+  unsigned bx = 32;
+  while (bx < p.row_vecs && bx < (unsigned)paged::kThreads) bx *= 2;
+  const unsigned by = paged::kThreads / bx;
+  const int64_t gx = (tokens + by * paged::kTokens - 1) / (by * paged::kTokens);
+  const int64_t gy = (p.row_vecs + bx - 1) / bx;
+  JO_REQUIRE(gy < 65536, JO_ERR_INVALID, "paged_kv_write: too many elements in a token");
+  paged::write_kernel<<<dim3((unsigned)gx, (unsigned)gy), dim3(bx, by), 0, static_cast<cudaStream_t>(stream)>>>(p);
   return check_launch("paged_kv_write");
 }
 

@@ -17,10 +17,11 @@
 //   warp 9       MMA issuer: S_t = Q_t K^T, O_t += P_t V on tcgen05, in the order
 //                PV0 QK0' PV1 QK1' so that the softmax of one tile overlaps the
 //                MMAs of the other, across items too
-//   warps 10-11  look after V in steps where some row does not see every key:
+//   warp 10      looks after V in steps where some row does not see every key:
 //                rows past the last visible key are zeroed (a product with P = 0
 //                would turn a NaN there into NaN), and a value row that only some
 //                rows may see is searched for NaN and infinities
+//   warp 11      walks the block's range and hands its pieces to the others
 //   warps 0-7    softmax: one thread per row, P over S in tensor memory
 // The running maximum only moves when it grows by more than 2^8, so most steps
 // leave O alone.
@@ -34,7 +35,7 @@ namespace vattn {
 constexpr int kRows = 128;               // rows of a tile
 constexpr int kKeys = 128;               // keys of a step
 constexpr int kThreads = 384;
-constexpr int kLead = 1;                 // steps that an item's beginning and end cost
+constexpr int kLead = 2;                 // steps that an item's beginning and end cost
 constexpr int kMin = 3;                  // steps of the shortest piece
 using Steps = Work<kKeys, kLead, kMin>;
 using Range = Steps::Range;
@@ -43,15 +44,34 @@ using Walk = Steps::Walk;
 
 __device__ int g_fault = 0;
 
+constexpr int kPieces = 8;               // pieces handed out ahead
+
+// A piece as the roles need it.
+struct Task {
+  int a, e;                              // steps [a, e); e < 0: the range's end
+  int end[2];                            // tile t takes part in steps [a, end[t])
+  int edge;                              // first step in which some row does not see every key
+  int tok, ntok;                         // the item's first token (absolute) and its tokens
+  int before;                            // keys before its first token (causal: token k sees before + k + 1)
+  int keys, kfirst;                      // the request's keys, and their first row where they are packed
+  int b, h;
+  int slot;                              // -1: the piece is a whole item, else the slot of its partial result
+  int pad[3];
+};
+
 template <int D> struct Cfg {
   static constexpr int HALVES = D / 64;
   static constexpr int HALF = kKeys * 128;                   // 128 rows x 64 elements
   static constexpr int TILE = HALVES * HALF;
   static constexpr int ST = D == 128 ? 2 : 4;                // K and V steps in flight
-  static constexpr int K0 = 2 * TILE, V0 = K0 + ST * TILE, BARS = V0 + ST * TILE;
-  enum : int { B_QF = 0, B_QE = 1, B_SF = 2, B_PF = 4, B_OF = 6, B_KF = 8, B_KE = B_KF + ST, B_VF = B_KE + ST,
-               B_VE = B_VF + ST, B_VG = B_VE + ST, B_END = B_VG + ST, B_N };
-  static constexpr int BYTES = BARS + 1024 /* barriers, flags */ + 1024 /* alignment */;
+  static constexpr int K0 = 2 * TILE, V0 = K0 + ST * TILE;
+  static constexpr int OUT = V0 + ST * TILE;                 // 2 KB of a softmax warp: 32 rows x 32 columns on their way out
+  static constexpr int TASKS = OUT + 8 * 2048;
+  static constexpr int BARS = TASKS + kPieces * (int)sizeof(Task);
+  enum : int { B_QF = 0, B_QE = 1, B_SF = 2, B_PF = 4, B_OF = 6, B_TF = 8, B_TE = B_TF + kPieces, B_KF = B_TE + kPieces,
+               B_KE = B_KF + ST, B_VF = B_KE + ST, B_VE = B_VF + ST, B_VG = B_VE + ST, B_END = B_VG + ST, B_N };
+  static constexpr int BYTES = BARS + 512 /* barriers, flags */ + 1024 /* alignment */;
+  static_assert(B_N * 8 + 8 + 4 * ST <= 512, "");
 };
 
 struct Maps {
@@ -62,16 +82,9 @@ struct Maps {
   Begun* begun;
 };
 
-// Steps [s.a, end) of a piece in which tile t takes part: none without rows, and
-// none after the last key that its rows see.
-__device__ __forceinline__ int tile_end(const Params& p, const Piece& s, int tpt, int t) {
-  const int tok = s.i * 2 * tpt, n = min(2 * tpt, s.r.n - tok);
-  if (t == 1) return n > tpt ? s.e : s.a;
-  return max(s.a, min(s.e, max(1, div_up(visible(p, s.r, tok + min(n, tpt) - 1), kKeys))));
-}
-// First step in which some row does not see every key.
-__device__ __forceinline__ int first_edge(const Params& p, const Piece& s, int tpt) {
-  return visible(p, s.r, s.i * 2 * tpt) / kKeys;
+// Keys that token k of the task's item sees.
+__device__ __forceinline__ int task_visible(const Params& p, const Task& t, int k) {
+  return p.causal ? max(0, t.before + k + 1) : t.keys;
 }
 
 // O (+)= P V for one row on the CUDA cores: the step's V holds a NaN or an
@@ -131,15 +144,20 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   __shared__ Steps::Near near;
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  Task* tasks = reinterpret_cast<Task*>(smem + C::TASKS);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::B_N);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* vflag = abort_flag + 1;  // [ST][2]: NaN or infinity found by each guard warp
+  volatile int* vflag = abort_flag + 1;  // [ST]: a NaN or infinity found in an edge step's V
   const uint32_t bar0 = smem_u32(bars);
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
 #define WAIT(i, parity, code) mbar_wait(BAR(i), (parity), abort_flag, &g_fault, (code))
+// The next task of a role that has had n of them.
+#define NEXT_TASK(n) (WAIT(C::B_TF + (n) % kPieces, ((n) / kPieces) & 1, 20))
+#define TASK(n) (tasks[(n) % kPieces])
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Request early = (int)threadIdx.x < p.batch ? request(p, threadIdx.x) : Request{0, 0, 0};
   launch_dependents();
   if (threadIdx.x == 0) {
     mbar_init(BAR(C::B_QF), 1);
@@ -150,97 +168,146 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       mbar_init(BAR(C::B_PF + t), 4);    // one arrival per softmax warp
       mbar_init(BAR(C::B_OF + t), 1);
     }
+    for (int s = 0; s < kPieces; ++s) {
+      mbar_init(BAR(C::B_TF + s), 1);
+      mbar_init(BAR(C::B_TE + s), 11);   // every warp but the one that hands them out
+    }
     for (int s = 0; s < ST; ++s) {
       mbar_init(BAR(C::B_KF + s), 1);
       mbar_init(BAR(C::B_KE + s), 1);
       mbar_init(BAR(C::B_VF + s), 1);
       mbar_init(BAR(C::B_VE + s), 1);
-      mbar_init(BAR(C::B_VG + s), 2);    // one arrival per guard warp
+      mbar_init(BAR(C::B_VG + s), 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_map(&maps.q);
+    tma_prefetch_map(&maps.k);
+    tma_prefetch_map(&maps.v);
+  }
   if (warp == 9) tmem_alloc_512(smem_u32(tmem_slot));
   Range range;
-  Steps::find<kThreads / 32>(p, 2 * maps.tpt, blockIdx.x, gridDim.x, scan, near, range);
+  Steps::find<kThreads / 32>(p, early, 2 * maps.tpt, blockIdx.x, gridDim.x, scan, near, range);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t sq = smem_u32(smem), sk = sq + C::K0, sv = sq + C::V0;
   const int tpt = maps.tpt;
-  Walk walk(p, 2 * tpt, near, range);
-  Piece s;
 
-  if (warp == 8) {
+  if (warp == 11) {
+    // ------------------------------------------------------ hands out pieces --
+    if (lane == 0) {
+      Walk walk(p, 2 * tpt, near, range);
+      Piece s;
+      Begun begun{0, 0, 0, 0};
+      bool more = true;
+      for (uint32_t n = 0; more; ++n) {
+        if (!WAIT(C::B_TE + n % kPieces, ((n / kPieces) & 1) ^ 1, 21)) {
+          begun.later = 0;
+          break;
+        }
+        more = walk.next(s);
+        Task t;
+        t.a = 0;
+        t.e = -1;
+        if (more) {
+          const int tok = s.i * 2 * tpt;
+          t.a = s.a;
+          t.e = s.e;
+          t.tok = s.r.first + tok;
+          t.ntok = min(2 * tpt, s.r.n - tok);
+          t.before = s.r.keys - s.r.n + tok;
+          t.keys = s.r.keys;
+          t.kfirst = s.r.first;
+          t.b = s.b;
+          t.h = s.h;
+          t.edge = task_visible(p, t, 0) / kKeys;
+          t.end[0] = max(s.a, min(s.e, max(1, div_up(task_visible(p, t, min(t.ntok, tpt) - 1), kKeys))));
+          t.end[1] = t.ntok > tpt ? s.e : s.a;
+          t.slot = s.whole() ? -1 : 2 * blockIdx.x + (s.a == 0);
+          if (s.a == 0 && s.e < s.steps)       // only the last piece ends inside an item
+            begun = Begun{Steps::later_blocks(range, s, blockIdx.x), t.tok, t.ntok, t.h};
+        }
+        TASK(n) = t;
+        mbar_arrive(BAR(C::B_TF + n % kPieces));
+      }
+      if (maps.begun) maps.begun[blockIdx.x] = begun;
+    }
+  } else if (warp == 8) {
     // ------------------------------------------------------------- producer --
     const int boxes = kKeys / maps.box;
     const int bx = lane % boxes, half = lane / boxes;         // this lane's copy of a step
     const bool mine = lane < boxes * C::HALVES;
     const uint32_t dst = half * C::HALF + bx * maps.box * 128;
-    uint32_t it = 0, pieces = 0;
-    bool ok = true;
-    if (lane == 0) {
-      tma_prefetch_map(&maps.q);
-      tma_prefetch_map(&maps.k);
-      tma_prefetch_map(&maps.v);
-    }
-    uint32_t v_issued = 0;
-    while (ok && walk.next(s)) {
-      int z16 = 0, w16 = 0;
-      for (int j = s.a; j < s.e && ok; ++j, ++it) {
-        // places of 16 keys each, four steps at a time: pages are multiples of 16 keys
-        const int ahead = (j - s.a) & 3;
-        if (ahead == 0) kv_place(p, s.r, s.b, j * kKeys + lane * 16, z16, w16);
-        const int from = (ahead * 8 + bx * (maps.box / 16)) & 31;
-        const int z = __shfl_sync(0xffffffffu, z16, from), w = __shfl_sync(0xffffffffu, w16, from);
+    uint32_t it = 0, v_issued = 0, n = 0;
+    for (;; ++n) {
+      if (!__all_sync(0xffffffffu, NEXT_TASK(n))) break;
+      const Task t = TASK(n);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(C::B_TE + n % kPieces));
+      if (t.e < 0) break;
+      // Places of 16 keys each (pages are multiples of 16 keys), four steps at a
+      // time; those of the next four are looked up meanwhile.
+      int z0 = 0, w0 = 0, z1, w1;
+      kv_place(p, t.kfirst, t.keys, t.b, t.a * kKeys + lane * 16, z1, w1);
+      bool ok = true;
+      for (int j = t.a; j < t.e; ++j, ++it) {
+        const int ahead = (j - t.a) & 3;
+        if (ahead == 0) {
+          z0 = z1;
+          w0 = w1;
+          kv_place(p, t.kfirst, t.keys, t.b, (j + 4) * kKeys + lane * 16, z1, w1);
+        }
+        const int from = ahead * 8 + bx * (maps.box / 16);
+        const int z = __shfl_sync(0xffffffffu, z0, from), w = __shfl_sync(0xffffffffu, w0, from);
         const int st = it % ST;
         const uint32_t ph = (it / ST) & 1;
-        ok = WAIT(C::B_KE + st, ph ^ 1, 1);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        ok = __all_sync(0xffffffffu, WAIT(C::B_KE + st, ph ^ 1, 1));
+        if (!ok) break;
         if (lane == 0) mbar_expect_tx(BAR(C::B_KF + st), C::TILE);
         __syncwarp();
-        if (mine) tma_load_4d(sk + st * C::TILE + dst, &maps.k, half * 64, s.h, z, w, BAR(C::B_KF + st));
-        if (j == s.a) {
-          ok = WAIT(C::B_QE, (pieces & 1) ^ 1, 2);
-          if (!__all_sync(0xffffffffu, ok)) {
+        if (mine) tma_load_4d(sk + st * C::TILE + dst, &maps.k, half * 64, t.h, z, w, BAR(C::B_KF + st));
+        if (j == t.a) {
+          ok = __all_sync(0xffffffffu, WAIT(C::B_QE, (n & 1) ^ 1, 2));
+          if (!ok) {
             ++it;
             break;
           }
-          const int tok = s.i * 2 * tpt, tiles = s.r.n - tok > tpt ? 2 : 1;
+          const int tiles = t.ntok > tpt ? 2 : 1;
           if (lane == 0) mbar_expect_tx(BAR(C::B_QF), tiles * D * 2 * p.group * tpt);
           __syncwarp();
           if (lane < tiles * C::HALVES) {
-            const int t = lane / C::HALVES, hf = lane % C::HALVES;
-            tma_load_4d(sq + t * C::TILE + hf * C::HALF, &maps.q, hf * 64, 0, s.h, s.r.first + tok + t * tpt,
-                        BAR(C::B_QF));
+            const int tl = lane / C::HALVES, hf = lane % C::HALVES;
+            tma_load_4d(sq + tl * C::TILE + hf * C::HALF, &maps.q, hf * 64, 0, t.h, t.tok + tl * tpt, BAR(C::B_QF));
           }
-          ++pieces;
         }
-        ok = WAIT(C::B_VE + st, ph ^ 1, 3);
-        if (!__all_sync(0xffffffffu, ok)) {
+        ok = __all_sync(0xffffffffu, WAIT(C::B_VE + st, ph ^ 1, 3));
+        if (!ok) {
           ++it;
           break;
         }
         if (lane == 0) mbar_expect_tx(BAR(C::B_VF + st), C::TILE);
         __syncwarp();
-        if (mine) tma_load_4d(sv + st * C::TILE + dst, &maps.v, half * 64, s.h, z, w, BAR(C::B_VF + st));
+        if (mine) tma_load_4d(sv + st * C::TILE + dst, &maps.v, half * 64, t.h, z, w, BAR(C::B_VF + st));
         v_issued = it + 1;
       }
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!ok) break;
     }
     // Every copy issued lands before the block leaves.
     if (lane == 0) {
       for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i) mbar_drain(BAR(C::B_KF + i % ST), (i / ST) & 1);
       for (uint32_t i = v_issued > ST ? v_issued - ST : 0; i < v_issued; ++i)
         mbar_drain(BAR(C::B_VF + i % ST), (i / ST) & 1);
-      if (pieces) mbar_drain(BAR(C::B_QF), (pieces - 1) & 1);
+      if (n) mbar_drain(BAR(C::B_QF), (n - 1) & 1);
     }
   } else if (warp == 9) {
     // ----------------------------------------------------------- MMA issuer --
     if (lane == 0) {
-      constexpr uint32_t ID_QK = instr_desc<T>(kRows, kKeys, false);
+      const uint32_t ID_QK = instr_desc<T>(kRows, kKeys, false) | (p.negate ? 1u << 13 : 0u);   // bit 13: -A
       constexpr uint32_t ID_PV = instr_desc<T>(kRows, D, true);
       auto qk = [&](int t, int st) {     // S_t = Q_t K^T
 #pragma unroll
@@ -257,37 +324,50 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           mma_ts(tmem + 128 * t, tmem + 256 + 128 * t + kk * 8, smem_desc(sv + st * C::TILE + kk * 2048, C::HALF),
                  ID_PV, (acc || kk != 0) ? 1u : 0u);
       };
-      uint32_t it = 0, pieces = 0, seen[2] = {0, 0};
-      bool more = walk.next(s), ok = true;
-      int j = 0, end[2] = {0, 0};
-      if (more) {
-        j = s.a;
-        end[0] = tile_end(p, s, tpt, 0);
-        end[1] = tile_end(p, s, tpt, 1);
+      uint32_t it = 0, n = 0, seen[2] = {0, 0};
+      uint32_t guarded = 0;              // parity of each place's guarded steps
+      bool ok = NEXT_TASK(0);
+      int a = 0, e = -1, end[2] = {0, 0}, edge = 0;
+      if (ok) {
+        const Task& t = TASK(0);
+        a = t.a, e = t.e, end[0] = t.end[0], end[1] = t.end[1], edge = t.edge;
+        mbar_arrive(BAR(C::B_TE));
+      }
+      bool more = e >= 0;
+      int j = a;
+      if (ok && more) {
         ok = WAIT(C::B_QF, 0, 4) && WAIT(C::B_KF, 0, 5);
         if (ok) {
           fence_after();
           for (int t = 0; t < 2; ++t)
             if (j < end[t]) qk(t, 0);
           mma_commit(BAR(C::B_KE));
-          if (j + 1 == s.e) mma_commit(BAR(C::B_QE));
+          if (j + 1 == e) mma_commit(BAR(C::B_QE));
         }
       }
       while (more && ok) {
-        Piece ns = s;
-        int nj = j + 1;
-        const bool turn = nj == s.e;     // the next step begins another piece
-        int nend[2] = {end[0], end[1]};
+        // the step after this one
+        int na = a, ne = e, nj = j + 1, nend[2] = {end[0], end[1]}, nedge = edge;
+        const bool turn = nj == e;       // it begins another piece
         if (turn) {
-          more = walk.next(ns);
-          nj = ns.a;
-          nend[0] = tile_end(p, ns, tpt, 0);
-          nend[1] = tile_end(p, ns, tpt, 1);
-          ++pieces;
+          ++n;
+          ok = NEXT_TASK(n);
+          if (!ok) break;
+          const Task& t = TASK(n);
+          na = t.a, ne = t.e, nend[0] = t.end[0], nend[1] = t.end[1], nedge = t.edge;
+          mbar_arrive(BAR(C::B_TE + n % kPieces));
+          more = ne >= 0;
+          nj = na;
         }
         const int st = it % ST, nst = (it + 1) % ST;
-        if (!WAIT(C::B_VG + st, (it / ST) & 1, 6)) break;
-        const bool careful = vflag[2 * st] | vflag[2 * st + 1];
+        bool careful = false;
+        if (j < edge) {
+          if (!WAIT(C::B_VF + st, (it / ST) & 1, 6)) break;
+        } else {
+          if (!WAIT(C::B_VG + st, (guarded >> st) & 1, 15)) break;
+          guarded ^= 1u << st;
+          careful = vflag[st];
+        }
         bool waited = false;
         for (int t = 0; t < 2 && ok; ++t) {
           if (j < end[t]) {
@@ -295,13 +375,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             if (!ok) break;
             ++seen[t];
             fence_after();
-            if (!careful) pv(t, st, j > s.a);
+            if (!careful) pv(t, st, j > a);
             if (j + 1 == end[t]) mma_commit(BAR(C::B_OF + t));
           }
           if (t == 1) mma_commit(BAR(C::B_VE + st));
           if (more && nj < nend[t]) {
             if (!waited) {
-              ok = (!turn || WAIT(C::B_QF, pieces & 1, 9)) && WAIT(C::B_KF + nst, ((it + 1) / ST) & 1, 10);
+              ok = (!turn || WAIT(C::B_QF, n & 1, 9)) && WAIT(C::B_KF + nst, ((it + 1) / ST) & 1, 10);
               if (!ok) break;
               fence_after();
               waited = true;
@@ -312,62 +392,66 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         if (!ok) break;
         if (more) {
           mma_commit(BAR(C::B_KE + nst));
-          if (nj + 1 == ns.e) mma_commit(BAR(C::B_QE));
+          if (nj + 1 == ne) mma_commit(BAR(C::B_QE));
         }
-        s = ns;
-        j = nj;
-        end[0] = nend[0];
-        end[1] = nend[1];
+        a = na, e = ne, j = nj, end[0] = nend[0], end[1] = nend[1], edge = nedge;
         ++it;
       }
       // Every MMA issued completes before tensor memory is freed.
       mma_commit(BAR(C::B_END));
       mbar_drain(BAR(C::B_END), 0);
     }
-  } else if (warp >= 10) {
-    // --------------------------------------------------------- guards of V --
-    const int g = warp - 10;
+  } else if (warp == 10) {
+    // ---------------------------------------------------------- guard of V --
     uint32_t it = 0;
-    bool ok = true;
-    Begun begun{0, 0, 0, 0};
-    while (ok && walk.next(s)) {
-      const int tok = s.i * 2 * tpt, edge = first_edge(p, s, tpt);
-      if (s.a == 0 && s.e < s.steps)     // only the last piece ends inside an item
-        begun = Begun{Steps::later_blocks(range, s, blockIdx.x), s.r.first + tok, min(2 * tpt, s.r.n - tok), s.h};
-      const int some = visible(p, s.r, tok);                                  // seen by every row
-      const int most = visible(p, s.r, min(s.r.n, tok + 2 * tpt) - 1);        // seen by any
-      for (int j = s.a; j < s.e; ++j, ++it) {
+    for (uint32_t n = 0;; ++n) {
+      if (!__all_sync(0xffffffffu, NEXT_TASK(n))) break;
+      const Task t = TASK(n);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(C::B_TE + n % kPieces));
+      if (t.e < 0) break;
+      const int some = task_visible(p, t, 0), most = task_visible(p, t, t.ntok - 1);   // seen by every row, by any
+      bool ok = true;
+      for (int j = t.a; j < t.e; ++j, ++it) {
         const int st = it % ST;
         ok = __all_sync(0xffffffffu, WAIT(C::B_VF + st, (it / ST) & 1, 11));
         if (!ok) break;
-        int bad = 0;
-        if (j >= edge) {
-          unsigned char* v = smem + C::V0 + st * C::TILE;
-          const int lo = max(0, some - j * kKeys), hi = min(kKeys, max(0, most - j * kKeys));
-          constexpr int CH = D / 8;      // 16-byte vectors of a row
-          for (int i = lo * CH + g * 32 + lane; i < kKeys * CH; i += 64) {
-            const int row = i / CH, col = (i % CH) * 8;
-            uint4* x = reinterpret_cast<uint4*>(v + swizzled(row, col, C::HALF));
-            if (row >= hi) {
-              *x = make_uint4(0, 0, 0, 0);
-            } else {
-              constexpr uint32_t E = Bits16<T>::kInf * 0x10001u, EL = Bits16<T>::kInf, EH = EL << 16;
-              const uint4 y = *x;
-              const uint32_t w[4] = {y.x & E, y.y & E, y.z & E, y.w & E};
+        if (j < t.edge) continue;
+        // Rows lo.. are searched (a few more below them do no harm), rows hi.. zeroed.
+        // Eight rows at a time, all loads before their use: at one load at a time
+        // this took four steps' time.
+        const int lo = max(0, some - j * kKeys), hi = min(kKeys, max(0, most - j * kKeys));
+        constexpr int CH = D / 8, STEP = 32 / CH;      // 16-byte vectors of a row; rows of one load of the warp
+        const int col = lane % CH, row0 = lane / CH;
+        unsigned char* v = smem + C::V0 + st * C::TILE + (col >> 3) * C::HALF;
+        uint32_t top = 0;
+        for (int r8 = lo & ~7; r8 < kKeys; r8 += 8) {
+          uint4 y[8 / STEP];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) bad |= (w[q] & EL) == EL || (w[q] & EH) == EH;
+          for (int k = 0; k < 8 / STEP; ++k) {
+            const int r = k * STEP + row0;             // row & 7
+            uint4* x = reinterpret_cast<uint4*>(v + (r8 + r) * 128 + (((col & 7) ^ r) << 4));
+            if (r8 + r < hi) {
+              y[k] = *x;
+            } else {
+              y[k] = make_uint4(0, 0, 0, 0);
+              *x = y[k];
             }
           }
-          fence_async_smem();
+#pragma unroll
+          for (int k = 0; k < 8 / STEP; ++k)
+            top = absmax2(absmax2(absmax2(absmax2(top, y[k].x), y[k].y), y[k].z), y[k].w);
         }
+        int bad = absmax2_fold(top) >= Bits16<T>::kInf;
+        fence_async_smem();
         bad = __any_sync(0xffffffffu, bad);
         if (lane == 0) {
-          vflag[2 * st + g] = bad;
+          vflag[st] = bad;
           mbar_arrive(BAR(C::B_VG + st));
         }
       }
+      if (!ok) break;
     }
-    if (g == 0 && lane == 0 && maps.begun) maps.begun[blockIdx.x] = ok ? begun : Begun{0, 0, 0, 0};
   } else {
     // -------------------------------------------------------------- softmax --
     const int t = warp >> 2;                       // tile of this warpgroup
@@ -376,17 +460,20 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const uint32_t tS = tmem + 256 + t * 128 + lane_off;
     const uint32_t tO = tmem + t * 128 + lane_off;
     const float c = p.scale_log2;
-    const int row_tok = row / p.group, row_head = row - row_tok * p.group;
-    uint32_t it = 0, tiles = 0, outs = 0;
-    bool ok = true;
-    while (ok && walk.next(s)) {
-      const int i_tok = s.i * 2 * tpt + t * tpt + row_tok;
-      const bool valid = row_tok < tpt && i_tok < s.r.n;
-      const int limit = visible(p, s.r, min(i_tok, s.r.n - 1));
-      const int end = tile_end(p, s, tpt, t), first = first_edge(p, s, tpt);
+    const int row_tok = row / p.group;             // of this row, in its tile
+    uint32_t it = 0, tiles = 0, outs = 0, guarded = 0;
+    for (uint32_t n = 0;; ++n) {
+      if (!__all_sync(0xffffffffu, NEXT_TASK(n))) break;
+      const Task& task = TASK(n);
+      if (task.e < 0) break;
+      const int a = task.a, e = task.e, end = task.end[t], first = task.edge;
+      const int k_tok = t * tpt + row_tok;         // the row's token in the item
+      const int limit = task_visible(p, task, min(k_tok, task.ntok - 1));
       float m = kNoMax;                            // running max of s * c (may lag the true one by less than 8)
       float l = 0.f;                               // running sum
-      for (int j = s.a; j < s.e; ++j, ++it) {
+      bool ok = true;
+      for (int j = a; j < e; ++j, ++it) {
+        if (j >= first) guarded ^= 1u << (it % ST);
         if (j >= end) continue;
         ok = __all_sync(0xffffffffu, WAIT(C::B_SF + t, tiles & 1, 12));
         if (!ok) break;
@@ -397,10 +484,6 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, xu + q * 32);
         tmem_wait_ld();
-        if (p.negate) {
-#pragma unroll
-          for (int i = 0; i < 128; ++i) x[i] = -x[i];
-        }
         const bool edge = j >= first;
         const int lim = limit - j * kKeys;
         if (edge) {
@@ -428,11 +511,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           uint32_t pk[16];
 #pragma unroll
           for (int i = 32 * ch; i < 32 * ch + 32; i += 2) {
-            float2 e = fma2(make_float2(x[i], x[i + 1]), c2, mn2);
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            pk[(i - 32 * ch) >> 1] = pack2<T>(e.x, e.y);
-            ra[(i >> 1) & 3] = add2(ra[(i >> 1) & 3], e);
+            float2 w = fma2(make_float2(x[i], x[i + 1]), c2, mn2);
+            w.x = ex2(w.x);
+            w.y = ex2(w.y);
+            pk[(i - 32 * ch) >> 1] = pack2<T>(w.x, w.y);
+            ra[(i >> 1) & 3] = add2(ra[(i >> 1) & 3], w);
           }
           tmem_st16(tS + 16 * ch, pk);
         }
@@ -440,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         l = __fmaf_rn(l, alpha, (r01.x + r01.y) + (r23.x + r23.y));
         // O_t *= alpha (PV_t of the step before has completed: it was issued
         // before the QK_t that released this S).
-        if (any_need && j > s.a) {
+        if (any_need && j > a) {
 #pragma unroll 1
           for (int q = 0; q < D; q += 32) {
             uint32_t o[32];
@@ -454,10 +537,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         tmem_wait_st();
         if (edge) {
           const int st = it % ST;
-          ok = __all_sync(0xffffffffu, WAIT(C::B_VG + st, (it / ST) & 1, 13));
+          ok = __all_sync(0xffffffffu, WAIT(C::B_VG + st, (~guarded >> st) & 1, 13));
           if (!ok) break;
-          if (vflag[2 * st] | vflag[2 * st + 1])
-            careful_pv<T, D>(tS, tO, smem + C::V0 + st * C::TILE, j == s.a, lim);
+          if (vflag[st]) careful_pv<T, D>(tS, tO, smem + C::V0 + st * C::TILE, j == a, lim);
         }
         fence_before();
         __syncwarp();
@@ -465,40 +547,52 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       }
       if (!ok) break;
       // ---- epilogue ----
-      const bool has = end > s.a;
+      const bool has = end > a;
       if (has) {
-        ok = __all_sync(0xffffffffu, WAIT(C::B_OF + t, outs & 1, 14));
-        if (!ok) break;
+        if (!__all_sync(0xffffffffu, WAIT(C::B_OF + t, outs & 1, 14))) break;
         ++outs;
         fence_after();
       }
-      if (s.whole()) {
-        if (!has) continue;
-        // a row that sees no key has l = 0 and an O that was never scaled: zero
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        T* orow = static_cast<T*>(p.out) + (int64_t)(s.r.first + i_tok) * p.o_ts +
-                  (int64_t)(s.h * p.group + row_head) * p.o_hs;
+      const bool valid = row_tok < tpt && k_tok < task.ntok;
+      if (task.slot < 0) {
+        if (has) {
+          // Through shared memory, so that a warp's store covers rows of 64 bytes
+          // and not single 16-byte pieces of 32 of them.
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const int row_head = row - row_tok * p.group;
+          const long long at = valid ? (long long)(task.tok + k_tok) * p.o_ts + (long long)(task.h * p.group + row_head) * p.o_hs
+                                     : -1;
+          long long to[4];               // rows that this lane stores a piece of
+#pragma unroll
+          for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, at, 8 * k + (lane >> 2));
+          unsigned char* buf = smem + C::OUT + warp * 2048;
 #pragma unroll 1
-        for (int q = 0; q < D; q += 32) {
-          uint32_t o[32];
-          tmem_ld32(tO + q, o);
-          tmem_wait_ld();
-          if (valid) {
-            uint4* dst = reinterpret_cast<uint4*>(orow + q);
+          for (int q = 0; q < D; q += 32) {
+            uint32_t o[32];
+            tmem_ld32(tO + q, o);
+            tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t w[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const float lo = __uint_as_float(o[8 * i + 2 * k]), hi = __uint_as_float(o[8 * i + 2 * k + 1]);
-                w[k] = l == 0.f ? 0u : pack2<T>(lo * inv, hi * inv);
+                w[k] = l == 0.f ? 0u : pack2<T>(lo * inv, hi * inv);    // a row that sees no key is zero
               }
-              dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(buf + lane * 64 + ((i ^ (lane >> 1) & 3) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int r = 8 * k + (lane >> 2), i = lane & 3;
+              const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 64 + ((i ^ (r >> 1) & 3) << 4));
+              if (to[k] >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to[k] + q + i * 8) = w;
+            }
+            __syncwarp();
           }
         }
       } else {
-        Slot<D, 2 * kRows>& slot = static_cast<Slot<D, 2 * kRows>*>(maps.partial)[2 * blockIdx.x + (s.a == 0 ? 1 : 0)];
+        Slot<D, 2 * kRows>& slot = static_cast<Slot<D, 2 * kRows>*>(maps.partial)[task.slot];
         const int r2 = t * kRows + row;
         slot.ml[r2] = make_float2(m, l);
         if (has) {
@@ -516,14 +610,22 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(C::B_TE + n % kPieces));
     }
   }
+
+  // Where this kernel began before the ones ahead of it had ended (see launch), it
+  // does not end before them.
+  wait_for_primary();
   fence_before();
   __syncthreads();
   fence_after();
   if (warp == 9) tmem_free_512(tmem);
 #undef BAR
 #undef WAIT
+#undef NEXT_TASK
+#undef TASK
 }
 
 // ------------------------------------------------------------------- host --
@@ -534,8 +636,7 @@ static int64_t tile_workspace(int head_dim) {
          2 * (int64_t)n * (int64_t)(head_dim == 64 ? sizeof(Slot<64, 2 * kRows>) : sizeof(Slot<128, 2 * kRows>));
 }
 static int64_t workspace_bytes_for(int head_dim) {
-  const int64_t a = tile_workspace(head_dim), b = few_workspace(head_dim);
-  return a > b ? a : b;
+  return tile_workspace(head_dim) + few_workspace(head_dim);
 }
 
 static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
@@ -574,7 +675,7 @@ static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int
 }
 
 template <typename T, int D>
-static int launch_tiles(const char* what, const Params& p, void* workspace, cudaStream_t stream) {
+static int launch_tiles(const char* what, const Params& p, void* workspace, bool overlap, cudaStream_t stream) {
   constexpr bool bf16 = IsBf16<T>::v;
   Maps maps;
   maps.tpt = kRows / p.group;
@@ -597,17 +698,27 @@ static int launch_tiles(const char* what, const Params& p, void* workspace, cuda
       return check_launch(what);
     attr[dev] = true;
   }
-  tile_kernel<T, D><<<blocks, kThreads, Cfg<D>::BYTES, stream>>>(maps, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<D>::BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = overlap ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, tile_kernel<T, D>, maps, p) != cudaSuccess) return check_launch(what);
   if (split) launch_join<T, D, 2 * kRows, kRows, 1>(p, maps.partial, maps.begun, maps.tpt, blocks, stream);
   return check_launch(what);
 }
 
-static int launch_all_tiles(const char* what, const Params& p, int dtype, void* workspace, cudaStream_t s) {
+static int launch_all_tiles(const char* what, const Params& p, int dtype, void* workspace, bool overlap, cudaStream_t s) {
   if (dtype == JO_DTYPE_BF16)
-    return p.head_dim == 64 ? launch_tiles<__nv_bfloat16, 64>(what, p, workspace, s)
-                            : launch_tiles<__nv_bfloat16, 128>(what, p, workspace, s);
-  return p.head_dim == 64 ? launch_tiles<__half, 64>(what, p, workspace, s)
-                          : launch_tiles<__half, 128>(what, p, workspace, s);
+    return p.head_dim == 64 ? launch_tiles<__nv_bfloat16, 64>(what, p, workspace, overlap, s)
+                            : launch_tiles<__nv_bfloat16, 128>(what, p, workspace, overlap, s);
+  return p.head_dim == 64 ? launch_tiles<__half, 64>(what, p, workspace, overlap, s)
+                          : launch_tiles<__half, 128>(what, p, workspace, overlap, s);
 }
 
 static int launch(const char* what, Params& p, int64_t max_query_len, int dtype, void* workspace,
@@ -627,7 +738,7 @@ static int launch(const char* what, Params& p, int64_t max_query_len, int dtype,
   // both kinds, each kernel takes its own.
   p.min_rows = 1;
   p.max_rows = INT32_MAX;
-  if (!p.table) return launch_all_tiles(what, p, dtype, workspace, s);
+  if (!p.table) return launch_all_tiles(what, p, dtype, workspace, false, s);
   const int64_t longest = max_query_len < p.tokens ? (max_query_len > 1 ? max_query_len : 1) : p.tokens;
   if (p.group <= kFewRows && longest * p.group <= kFewRows)
     return launch_few(what, p, longest * p.group, dtype, workspace, s);
@@ -637,8 +748,11 @@ static int launch(const char* what, Params& p, int64_t max_query_len, int dtype,
     if (st != JO_OK) return st;
     p.min_rows = kFewRows + 1;
     p.max_rows = INT32_MAX;
+    // It needs nothing of what the kernel for few rows does, and has a workspace of
+    // its own: its blocks may begin as that one's end.
+    return launch_all_tiles(what, p, dtype, static_cast<char*>(workspace) + few_workspace(p.head_dim), true, s);
   }
-  return launch_all_tiles(what, p, dtype, workspace, s);
+  return launch_all_tiles(what, p, dtype, workspace, false, s);
 }
 
 }  // namespace vattn
@@ -659,7 +773,7 @@ int jo_paged_attention(const void* q, const void* key_cache, const void* value_c
   JO_REQUIRE(page_size >= 16 && page_size % 16 == 0 && page_size < (1LL << 30), JO_ERR_INVALID,
              "%s: page_size must be a multiple of 16 (got %lld)", what, (long long)page_size);
   JO_REQUIRE(num_blocks >= 0 && num_blocks < (1LL << 31) && table_width >= 0 && table_width < (1LL << 31) &&
-                 table_stride >= 0 && table_width * page_size < (1LL << 31),
+                 table_stride >= 0 && table_width * page_size <= (1LL << 30),
              JO_ERR_INVALID, "%s: invalid cache or block table shape", what);
   vattn::Params p{q, key_cache, value_cache, out, query_starts, kv_lens, block_tables,
                   r[0], r[1], c[0], c[1], c[2], c[3], c[4], c[5], r[2], r[3], table_stride};

@@ -62,9 +62,11 @@ __host__ __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1
 
 constexpr int kNear = 32;                // requests of a block's range that it keeps at hand
 
-// floor(a / b) for 0 <= a < 2^52, b > 0 (a 64-bit integer division takes some
-// hundreds of cycles, and every block's first copy waits for a few of them).
+// floor(a / b) for 0 <= a < 2^52, b > 0.  Every block's first copy waits for a few
+// of them: 32-bit divisions where the numbers allow, a 64-bit one takes hundreds
+// of cycles.
 __device__ __forceinline__ long long div_floor(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
   long long q = (long long)((double)a / (double)b);
   if (q * b > a) --q;
   if ((q + 1) * b <= a) ++q;
@@ -134,22 +136,25 @@ struct Work {
 
   // Range of block c of at most C.  All threads of the block (WARPS warps) take
   // part, each looking after one request of a run of as many as there are threads.
-  // Latency-bound: one look at the lengths, a scan over the block, two divisions.
+  // Latency-bound: one look at the lengths (`early`: the one of the first run, asked
+  // for as early as possible), a scan over the block, a few divisions.
   template <int WARPS>
-  static __device__ void find(const Params& p, int tpi, int c, int C, Scan<WARPS>& s, Near& near, Range& range) {
+  static __device__ void find(const Params& p, const Request& early, int tpi, int c, int C, Scan<WARPS>& s, Near& near,
+                              Range& range) {
     constexpr int THREADS = 32 * WARPS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool one = p.batch <= THREADS; // one run holds them all
     Cuts cuts;
     long long begin = 0, end = 0;
+    if (threadIdx.x < 2) s.cut[threadIdx.x] = Place{p.batch, 0, 0, 1, -1, {0, 0, 0}, 0, 0, 0};
     // First time round: the number of units, and where one run holds all the
     // cuts too.  Second: the cuts.
     for (int round = one ? 1 : 0; round < 2; ++round) {
       longlong2 base = make_longlong2(0, 0);
       for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
         const int b = b0 + threadIdx.x;
-        Request r{0, 0, 0};
-        if (b < p.batch) r = request(p, b);
+        Request r = early;
+        if (b0 > 0) r = b < p.batch ? request(p, b) : Request{0, 0, 0};
         long long u = 0;
         const bool many = r.n > 16 * tpi; // too many items for one thread
         if (!many) u = head_units(p, r, tpi, 0, 1);
@@ -185,10 +190,6 @@ struct Work {
           begin = cuts.at(c);
           end = cuts.at(c + 1);
         }
-        if (b0 == 0) {
-          if (threadIdx.x < 2) s.cut[threadIdx.x] = Place{p.batch, 0, 0, 1, end, {0, 0, 0}, 0, 0, 0};
-          __syncthreads();
-        }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const long long t = k ? end : begin;
@@ -218,16 +219,20 @@ struct Work {
     // head, item and step of the two cuts, a warp for each
     if (warp < 2 && s.cut[warp].b < p.batch) {
       Place& f = s.cut[warp];
-      const int h = (int)div_floor(f.off, f.per_head), ni = div_up(f.r.n, tpi);
-      long long off = f.off - h * f.per_head;
-      for (int q0 = 0; q0 < ni; q0 += 32) {
-        const int q = q0 + lane, n = q < ni ? steps(p, f.r, q, tpi) : 0;
-        long long inc = q < ni ? LEAD + n : 0;
-        const long long u = inc;
+      const Request r = f.r;
+      const int h = (int)div_floor(f.off, f.per_head);
+      long long off = f.off - h * f.per_head;                // units into the key head's items
+      for (int q0 = 0;; q0 += 32) {
+        const int q = q0 + lane;
+        const int n = (long long)q * tpi < r.n ? steps(p, r, q, tpi) : 0;
+        int inc = n ? LEAD + n : 0;      // (32 items of at most 2^24 + LEAD units)
+        const int u = inc;
+        if (r.n > tpi) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += x;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
+          }
         }
         const unsigned hit = __ballot_sync(0xffffffffu, inc > off);
         if (hit) {
@@ -246,6 +251,7 @@ struct Work {
           }
           break;
         }
+        if (q0 + 32LL >= r.n) break;     // (not reached: the cut lies in the request)
         off -= __shfl_sync(0xffffffffu, inc, 31);
       }
     }
@@ -267,7 +273,9 @@ struct Work {
     }
     __syncthreads();
     if (threadIdx.x == 0) near.next = near.count > 0 ? near.b[near.count - 1] + 1 : p.batch;
-    range = Range{s.cut[0].b, s.cut[0].h, s.cut[0].i, s.cut[0].step, s.cut[0].at, s.cut[1].at, cuts};
+    // a cut that falls into no request is the end of them all
+    range = Range{s.cut[0].b, s.cut[0].h, s.cut[0].i, s.cut[0].step, s.cut[0].at < 0 ? cuts.total : s.cut[0].at,
+                  s.cut[1].at < 0 ? cuts.total : s.cut[1].at, cuts};
   }
 
   // One block's stretch of one item.
@@ -484,17 +492,18 @@ inline bool kv_maps(const Params& p, bool bf16, int most, CUtensorMap* k, CUtens
   return make_map_4d(k, bf16, p.k, d, ks, kb) && make_map_4d(v, bf16, p.v, d, vs, kb);
 }
 
-// Coordinates (z, w) of key `key` in those maps; a block outside the cache, and
-// a key past the request's, read as zeros.
-__device__ __forceinline__ void kv_place(const Params& p, const Request& r, int b, int key, int& z, int& w) {
+// Coordinates (z, w) of key `key` of request b in those maps; a block outside the
+// cache, and a key past the request's, read as zeros.  first: the row of its first
+// key where keys are packed.
+__device__ __forceinline__ void kv_place(const Params& p, int first, int keys, int b, int key, int& z, int& w) {
   if (p.table) {
     const int pg = key / p.page;
     z = key - pg * p.page;
     int block = -1;
-    if (key < r.keys) block = p.table[(int64_t)b * p.table_stride + pg];
+    if (key < keys) block = p.table[(int64_t)b * p.table_stride + pg];
     w = block >= 0 && block < p.num_blocks ? block : -1;
   } else {
-    z = r.first + key;
+    z = first + key;
     w = 0;
   }
 }

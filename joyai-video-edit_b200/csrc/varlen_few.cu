@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
 #define FULL(s) (bar0 + 8u * (uint32_t)(s))
 #define EMPTY(s) (bar0 + 8u * (uint32_t)(ST + (s)))
 
+  const Request early = (int)threadIdx.x < p.batch ? request(p, threadIdx.x) : Request{0, 0, 0};
   launch_dependents();
   if (threadIdx.x == 0) {
     tma_prefetch_map(&maps.k);
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
   }
   Range range;
   using Scan = Steps::Scan<kThreads / 32>;
-  Steps::find<kThreads / 32>(p, maps.tpi, blockIdx.x, gridDim.x, *reinterpret_cast<Scan*>(smem), near, range);
+  Steps::find<kThreads / 32>(p, early, maps.tpi, blockIdx.x, gridDim.x, *reinterpret_cast<Scan*>(smem), near, range);
   fence_async_smem();                    // the scan's space becomes the ring
   __syncthreads();
   const int tpi = maps.tpi;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
       int z = 0, w = 0;                  // places of 16 keys each, eight steps at a time: pages are multiples of 16 keys
       for (int j = s.a; j < s.e; ++j, ++it) {
         const int st = it % ST, ahead = (j - s.a) & 7;
-        if (ahead == 0) kv_place(p, s.r, s.b, j * kKeys + lane * 16, z, w);
+        if (ahead == 0) kv_place(p, s.r.first, s.r.keys, s.b, j * kKeys + lane * 16, z, w);
         const int from = (ahead * 4 + bx * (maps.box / 16)) & 31;
         const int zz = __shfl_sync(0xffffffffu, z, from), ww = __shfl_sync(0xffffffffu, w, from);
         ok = __all_sync(0xffffffffu, mbar_wait(EMPTY(st), ((it / ST) & 1) ^ 1, abort_flag, &g_fault, 101));
@@ -206,11 +207,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
         const uint32_t ks = ring + st * 2 * C::TILE, vs = ks + C::TILE;
         const int key0 = j * kKeys + warp * 16;              // this warp's keys
         const uint32_t pbuf = ps + (it & 1) * C::P_BYTES;
-        float x[MT][2][4];
+        float x[MT][2][4], x2[MT][2][4];                     // even and odd products apart: half the chain
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int n = 0; n < 2; ++n) x[t][n][0] = x[t][n][1] = x[t][n][2] = x[t][n][3] = 0.f;
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[t][n][i] = x2[t][n][i] = 0.f;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           uint32_t b[4];
@@ -219,10 +222,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
           for (int t = 0; t < MT; ++t) {
             uint32_t a[4];
             ldsm4(qs + (t * 16 + arow) * D * 2 + (((k * 2 + acol) ^ (arow & 7)) << 4), a);
-            mma16816<T>(x[t][0], a, b[0], b[1]);
-            mma16816<T>(x[t][1], a, b[2], b[3]);
+            mma16816<T>(k & 1 ? x2[t][0] : x[t][0], a, b[0], b[1]);
+            mma16816<T>(k & 1 ? x2[t][1] : x[t][1], a, b[2], b[3]);
           }
         }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[t][n][i] += x2[t][n][i];
         const bool edge = (j + 1) * kKeys > some;            // some row does not see every key of this step
         int bad = 0;
         if (edge) {
@@ -235,19 +244,26 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
                 if (key0 + n * 8 + qc + (i & 1) >= limit[t][i >> 1]) x[t][n][i] = -INFINITY;
           // a product with a weight of 0 would turn a NaN in V into NaN: in this
           // warp's columns, keys that no row sees are zeroed, others are searched
-          unsigned char* v = smem + st * 2 * C::TILE + C::TILE;
-          for (int i = max(0, some - j * kKeys) * NW + lane; i < kKeys * NW; i += 32) {
-            const int row = i / NW;
-            uint4* y = reinterpret_cast<uint4*>(v + swizzled(row, (warp * NW + i % NW) * 8, C::HALF));
-            if (j * kKeys + row >= most) {
-              *y = make_uint4(0, 0, 0, 0);
-            } else {
-              constexpr uint32_t EL = Bits16<T>::kInf, EH = EL << 16;
-              const uint32_t u[4] = {y->x, y->y, y->z, y->w};
+          // (some rows below the first partly visible one are looked at too)
+          constexpr int STEP = 32 / NW;                      // rows of one load of the warp
+          const int col = warp * NW + lane % NW, row0 = lane / NW;
+          const int hi = most - j * kKeys;
+          unsigned char* v = smem + st * 2 * C::TILE + C::TILE + (col >> 3) * C::HALF;
+          uint32_t big = 0;
+          for (int r0 = max(0, some - j * kKeys) & ~(2 * STEP - 1); r0 < kKeys; r0 += 2 * STEP) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) bad |= (u[k] & EL) == EL || (u[k] & EH) == EH;
+            for (int k = 0; k < 2; ++k) {
+              const int r = r0 + k * STEP + row0;
+              uint4* y = reinterpret_cast<uint4*>(v + r * 128 + (((col ^ r) & 7) << 4));
+              if (r < hi) {
+                const uint4 u = *y;
+                big = absmax2(absmax2(absmax2(absmax2(big, u.x), u.y), u.z), u.w);
+              } else {
+                *y = make_uint4(0, 0, 0, 0);
+              }
             }
           }
+          bad = absmax2_fold(big) >= Bits16<T>::kInf;
           fence_async_smem();                                // the next copy into this place comes after these writes
           bad = __any_sync(0xffffffffu, bad);
         }
@@ -430,7 +446,7 @@ static int launch(const char* what, const Params& p, void* workspace, cudaStream
     attr[dev] = true;
   }
   few_kernel<T, D, MT><<<blocks, kThreads, C::BYTES, stream>>>(maps, p);
-  if (split) launch_join<T, D, 32, C::R, 8>(p, maps.partial, maps.begun, maps.tpi, blocks, stream);
+  if (split) launch_join<T, D, 32, C::R, 2>(p, maps.partial, maps.begun, maps.tpi, blocks, stream);
   return check_launch(what);
 }
 
