@@ -308,9 +308,11 @@ int jo_prompt_attention(const void* q, const void* k, const void* v, const int32
                         const int64_t* row_strides, const int64_t* kv_strides, int causal, float scale, int dtype,
                         void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Bytes of workspace that the two calls above need for these sizes (the
- * partial results of work that is split along the keys). */
-int jo_varlen_attention_workspace(int64_t tokens, int64_t heads, int64_t head_dim, int64_t* bytes);
+/* Bytes of workspace that the two calls above need on the current device for the
+ * partial results of work that is split along the keys (0: none, the pointer may
+ * be NULL).  max_keys: the most keys that a request can have, table_width *
+ * page_size or the number of packed rows. */
+int jo_varlen_attention_workspace(int64_t max_keys, int64_t head_dim, int64_t* bytes);
 
 /* Diagnostic: fault code left by a wait of the two calls above that timed out
  * (0 = none); reset != 0 clears it.  Synchronous. */

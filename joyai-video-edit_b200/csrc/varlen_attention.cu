@@ -635,9 +635,12 @@ static int64_t tile_workspace(int head_dim) {
   return begun_bytes(n) +
          2 * (int64_t)n * (int64_t)(head_dim == 64 ? sizeof(Slot<64, 2 * kRows>) : sizeof(Slot<128, 2 * kRows>));
 }
-static int64_t workspace_bytes_for(int head_dim) {
-  return tile_workspace(head_dim) + few_workspace(head_dim);
+// An item has a cut inside only if it is long enough to have one away from its edges.
+static bool tiles_split(int64_t max_keys) { return max_keys > (2 * kMin - 1) * kKeys; }
+static int64_t workspace_bytes_for(int64_t max_keys, int head_dim) {
+  return tiles_split(max_keys) || few_splits(max_keys) ? tile_workspace(head_dim) + few_workspace(head_dim) : 0;
 }
+static int64_t max_keys(const Params& p) { return p.table ? (int64_t)p.width * p.page : p.tokens; }
 
 static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
                  int64_t head_dim, float scale, int dtype) {
@@ -686,9 +689,7 @@ static int launch_tiles(const char* what, const Params& p, void* workspace, bool
     set_error("%s: cuTensorMapEncodeTiled failed", what);
     return JO_ERR_CUDA;
   }
-  // No item has a cut inside when none is long enough to have one away from its edges.
-  const int64_t most_keys = p.table ? (int64_t)p.width * p.page : p.tokens;
-  const bool split = most_keys > (2 * kMin - 1) * kKeys;
+  const bool split = tiles_split(max_keys(p));
   maps.begun = split ? static_cast<Begun*>(workspace) : nullptr;
   maps.partial = static_cast<char*>(workspace) + begun_bytes(blocks);
   static bool attr[kMaxDevices] = {};
@@ -727,8 +728,8 @@ static int launch(const char* what, Params& p, int64_t max_query_len, int dtype,
   JO_REQUIRE(p.q && p.out && p.starts, JO_ERR_INVALID, "%s: null tensor pointer", what);
   int st = require_sm100();
   if (st != JO_OK) return st;
-  const int64_t need = workspace_bytes_for(p.head_dim);
-  JO_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, JO_ERR_INVALID,
+  const int64_t need = workspace_bytes_for(max_keys(p), p.head_dim);
+  JO_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), JO_ERR_INVALID,
              "%s: a 16-byte aligned workspace of %lld bytes is needed (got %lld)", what, (long long)need,
              (long long)workspace_bytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -807,13 +808,12 @@ int jo_prompt_attention(const void* q, const void* k, const void* v, const int32
   return vattn::launch(what, p, tokens, dtype, workspace, workspace_bytes, stream);
 }
 
-int jo_varlen_attention_workspace(int64_t tokens, int64_t heads, int64_t head_dim, int64_t* bytes) {
+int jo_varlen_attention_workspace(int64_t max_keys, int64_t head_dim, int64_t* bytes) {
   using namespace jo;
   JO_REQUIRE(bytes, JO_ERR_INVALID, "varlen_attention_workspace: null pointer");
   JO_REQUIRE(head_dim == 64 || head_dim == 128, JO_ERR_INVALID,
              "varlen_attention_workspace: head_dim must be 64 or 128 (got %lld)", (long long)head_dim);
-  (void)tokens, (void)heads;
-  *bytes = vattn::workspace_bytes_for((int)head_dim);
+  *bytes = vattn::workspace_bytes_for(max_keys, (int)head_dim);
   return JO_OK;
 }
 

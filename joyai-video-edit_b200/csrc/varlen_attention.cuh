@@ -512,6 +512,7 @@ __device__ __forceinline__ void kv_place(const Params& p, int first, int keys, i
 // request as far as the host knows it; up to kFewRows it serves them best.
 constexpr int kFewRows = 32;
 int64_t few_workspace(int head_dim);
+bool few_splits(int64_t max_keys);     // whether an item of so many keys can have a cut inside
 int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, cudaStream_t stream);
 int few_last_fault(int reset);
 

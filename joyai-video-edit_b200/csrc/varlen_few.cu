@@ -434,8 +434,7 @@ static int launch(const char* what, const Params& p, void* workspace, cudaStream
   }
   const int blocks = kBlocksPerSm * sm_count();
   maps.tpi = C::R / p.group;
-  // no item has a cut inside when none is long enough to have one away from its edges
-  const bool split = (int64_t)p.width * p.page > (2 * kMin - 1) * kKeys;
+  const bool split = few_splits((int64_t)p.width * p.page);
   maps.begun = split ? static_cast<Begun*>(workspace) : nullptr;
   maps.partial = static_cast<char*>(workspace) + begun_bytes(blocks);
   static bool attr[kMaxDevices] = {};
@@ -456,6 +455,8 @@ static int launch_rows(const char* what, const Params& p, int64_t rows, void* wo
 }
 
 }  // namespace few
+
+bool few_splits(int64_t max_keys) { return max_keys > (2 * few::kMin - 1) * few::kKeys; }
 
 int64_t few_workspace(int head_dim) {
   const int n = few::kBlocksPerSm * sm_count();

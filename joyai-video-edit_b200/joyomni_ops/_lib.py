@@ -70,7 +70,7 @@ SIGNATURES = {
     "jo_paged_attention": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p,
                            _i32, _f32, _i64, _i32, _p, _i64, _p],
     "jo_prompt_attention": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i32, _f32, _i32, _p, _i64, _p],
-    "jo_varlen_attention_workspace": [_i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "jo_varlen_attention_workspace": [_i64, _i64, ctypes.POINTER(_i64)],
     "jo_varlen_attention_last_fault": [_i32],
     "jo_ipc_get_handle": [_p, _p, ctypes.POINTER(_i64)],
     "jo_ipc_open": [_p, ctypes.POINTER(_p)],

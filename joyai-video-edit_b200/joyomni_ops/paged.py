@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -28,8 +29,8 @@ from ._lib import check as _check, lib as _L
 
 _DT16 = {torch.float16: _lib.JO_DTYPE_F16, torch.bfloat16: _lib.JO_DTYPE_BF16}
 _I32, _I64 = torch.int32, torch.int64
-_S4 = ctypes.c_int64 * 4
-_S6 = ctypes.c_int64 * 6
+_S4 = struct.Struct("4q").pack        # strides for the C ABI's const int64_t*
+_S6 = struct.Struct("6q").pack
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch._C._cuda_getDevice
 
@@ -43,24 +44,15 @@ def _chk(cond: bool, msg: str) -> None:
         raise RuntimeError(msg)
 
 
-class _On:
-    """Makes device `idx` current for a call and gives its current stream."""
-
-    __slots__ = ("idx", "prev")
-
-    def __init__(self, idx: int):
-        self.idx = idx
-
-    def __enter__(self) -> int:
-        self.prev = _device()
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.idx)
-        return _stream(self.idx)
-
-    def __exit__(self, *exc):
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.prev)
-        return False
+def _call(f, idx: int, *args) -> None:
+    """f(*args, stream) on the current stream of device `idx`, which is current meanwhile."""
+    if _device() == idx:
+        status = f(*args, _stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            status = f(*args, _stream(idx))
+    if status:
+        _check(status)
 
 
 def _ints(t: torch.Tensor, name: str, dim: int, dtype: torch.dtype, idx: int) -> None:
@@ -126,11 +118,9 @@ def paged_layout(cached_lens, new_lens, block_tables, free_blocks, page_size: in
             and slots.is_contiguous() and pos.is_contiguous()):
         raise RuntimeError(f"out must hold contiguous tensors on cuda:{idx} of PagedLayout.empty({B}, {num_tokens}, ...)'s "
                            "sizes and types")
-    with _On(idx) as st:
-        _check(_L.jo_paged_layout(cached_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(),
-                                  free_blocks.data_ptr(), B, width, block_tables.stride(0) if B > 1 else width,
-                                  free_blocks.numel(), page_size, num_tokens, starts.data_ptr(), lens.data_ptr(),
-                                  slots.data_ptr(), pos.data_ptr(), needed.data_ptr(), st))
+    _call(_L.jo_paged_layout, idx, cached_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(),
+          free_blocks.data_ptr(), B, width, block_tables.stride(0) if B > 1 else width, free_blocks.numel(), page_size,
+          num_tokens, starts.data_ptr(), lens.data_ptr(), slots.data_ptr(), pos.data_ptr(), needed.data_ptr())
     return out
 
 
@@ -154,19 +144,18 @@ def paged_kv_write(key, value, key_cache, value_cache, slots) -> None:
     have the same slot."""
     idx, dt = key.get_device(), key.dtype
     code = _DT16.get(dt)
-    T, H, D = key.shape if key.dim() == 3 else (0, 0, 0)
+    shape, cs = key.shape, key_cache.shape
     a, b, c, d = key.stride(), value.stride(), key_cache.stride(), value_cache.stride()
-    if not (idx >= 0 and code is not None and key.dim() == 3 and key.shape == value.shape and key_cache.dim() == 4
-            and value_cache.shape == key_cache.shape and key_cache.shape[2:] == key.shape[1:] and value.dtype is dt
+    if not (idx >= 0 and code is not None and len(shape) == 3 and value.shape == shape and len(cs) == 4
+            and value_cache.shape == cs and cs[2:] == shape[1:] and value.dtype is dt
             and key_cache.dtype is dt and value_cache.dtype is dt and value.get_device() == idx
             and key_cache.get_device() == idx and value_cache.get_device() == idx and a[2] == b[2] == c[3] == d[3] == 1
-            and slots.dtype is _I64 and slots.get_device() == idx and slots.dim() == 1 and slots.is_contiguous()
-            and slots.numel() == T):
+            and slots.dtype is _I64 and slots.get_device() == idx and slots.is_contiguous() and slots.shape == shape[:1]):
         _refuse_write(key, value, key_cache, value_cache, slots)
-    with _On(idx) as st:
-        _check(_L.jo_paged_kv_write(key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-                                    slots.data_ptr(), T, H, D, key_cache.size(0), key_cache.size(1),
-                                    _S4(a[0], a[1], b[0], b[1]), _S6(c[0], c[1], c[2], d[0], d[1], d[2]), code, st))
+    T, H, D = shape
+    _call(_L.jo_paged_kv_write, idx, key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+          slots.data_ptr(), T, H, D, cs[0], cs[1], _S4(a[0], a[1], b[0], b[1]),
+          _S6(c[0], c[1], c[2], d[0], d[1], d[2]), code)
 
 
 def _refuse_write(key, value, key_cache, value_cache, slots) -> None:
@@ -185,33 +174,38 @@ def _refuse_write(key, value, key_cache, value_cache, slots) -> None:
 _ws_bytes = {}
 
 
-def varlen_attention_workspace(num_tokens: int, heads: int, head_dim: int) -> int:
-    """Bytes of workspace that paged_attention and prompt_attention use for
-    queries of these sizes (partial results of work that is split along the keys)."""
+def varlen_attention_workspace(max_keys: int, head_dim: int) -> int:
+    """Bytes of workspace that paged_attention and prompt_attention need on the
+    current device for the partial results of work that is split along the keys.
+    max_keys: the most keys that a request can have, block_tables' width times the
+    page size, or the number of packed rows."""
     n = ctypes.c_int64()
-    _check(_L.jo_varlen_attention_workspace(num_tokens, heads, head_dim, ctypes.byref(n)))
+    _check(_L.jo_varlen_attention_workspace(max_keys, head_dim, ctypes.byref(n)))
     return n.value
 
 
-def _workspace(workspace, T: int, H: int, D: int, q):
-    idx = q.get_device()
-    need = _ws_bytes.get((idx, T, H, D))
+def _workspace(workspace, idx: int, max_keys: int, D: int):
+    """(address, bytes, the tensor) of a call's workspace."""
+    need = _ws_bytes.get((idx, max_keys, D))
     if need is None:
         if len(_ws_bytes) > 4096:
             _ws_bytes.clear()
-        with _On(idx):
-            need = _ws_bytes[(idx, T, H, D)] = varlen_attention_workspace(T, H, D)
+        with torch.cuda.device(idx):
+            need = _ws_bytes[(idx, max_keys, D)] = varlen_attention_workspace(max_keys, D)
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=q.device), need
+        if need == 0:
+            return 0, 0, None
+        workspace = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", idx))
+        return workspace.data_ptr(), need, workspace
     have = workspace.numel() * workspace.element_size()
     _chk(workspace.get_device() == idx and workspace.is_contiguous() and have >= need,
          f"workspace must be a contiguous tensor of at least {need} bytes on cuda:{idx}")
-    return workspace, have
+    return workspace.data_ptr(), have, workspace
 
 
 def _out(q, out):
     if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format)
+        return torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     _chk(out.shape == q.shape, "out must have query's shape")
     _rows(out, "out", q.dtype, q.get_device())
     return out
@@ -243,30 +237,26 @@ def paged_attention(query, key_cache, value_cache, block_tables, query_starts, k
     call at a time; by default allocated per call."""
     idx, dt = query.get_device(), query.dtype
     code = _DT16.get(dt)
-    B = kv_lens.numel()
+    shape, cs, ts = query.shape, key_cache.shape, block_tables.shape
     a, c, d = query.stride(), key_cache.stride(), value_cache.stride()
-    if not (idx >= 0 and code is not None and query.dim() == 3 and key_cache.dim() == 4
-            and value_cache.shape == key_cache.shape and a[2] == c[3] == d[3] == 1 and key_cache.size(3) == query.size(2)
+    if not (idx >= 0 and code is not None and len(shape) == 3 and len(cs) == 4 and len(ts) == 2
+            and value_cache.shape == cs and a[2] == c[3] == d[3] == 1 and cs[3] == shape[2]
             and key_cache.dtype is dt and value_cache.dtype is dt and key_cache.get_device() == idx
             and value_cache.get_device() == idx and block_tables.dtype is _I32 and query_starts.dtype is _I32
             and kv_lens.dtype is _I32 and block_tables.get_device() == idx and query_starts.get_device() == idx
-            and kv_lens.get_device() == idx and block_tables.dim() == 2 and query_starts.dim() == kv_lens.dim() == 1
-            and block_tables.is_contiguous() and query_starts.is_contiguous() and kv_lens.is_contiguous()
-            and block_tables.size(0) == B and query_starts.numel() == B + 1):
+            and kv_lens.get_device() == idx and block_tables.is_contiguous() and query_starts.is_contiguous()
+            and kv_lens.is_contiguous() and kv_lens.shape == ts[:1] and query_starts.shape == (ts[0] + 1,)):
         _refuse_paged(query, key_cache, value_cache, block_tables, query_starts, kv_lens)
-    T, H, D = query.shape
+    T, H, D = shape
+    B, width = ts
     o = _out(query, out)
-    nb, page, Hk, _ = key_cache.shape
-    width = block_tables.size(1)
-    ws, ws_bytes = _workspace(workspace, T, H, D, query)
+    ws, ws_bytes, _keep = _workspace(workspace, idx, width * cs[1], D)
     e = o.stride()
-    with _On(idx) as st:
-        _check(_L.jo_paged_attention(
-            query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
-            query_starts.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), T, B, H, Hk, D, nb, page, width,
-            block_tables.stride(0) if B > 1 else width, _S4(a[0], a[1], e[0], e[1]),
-            _S6(c[0], c[1], c[2], d[0], d[1], d[2]), bool(causal), 1.0 / math.sqrt(D) if scale is None else scale,
-            T if max_query_len is None else max_query_len, code, ws.data_ptr(), ws_bytes, st))
+    _call(_L.jo_paged_attention, idx, query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+          block_tables.data_ptr(), query_starts.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), T, B, H, cs[2], D, cs[0],
+          cs[1], width, block_tables.stride(0) if B > 1 else width, _S4(a[0], a[1], e[0], e[1]),
+          _S6(c[0], c[1], c[2], d[0], d[1], d[2]), bool(causal), 1.0 / math.sqrt(D) if scale is None else scale,
+          T if max_query_len is None else max_query_len, code, ws, ws_bytes)
     return o
 
 
@@ -297,22 +287,21 @@ def prompt_attention(query, key, value, seq_starts, *, causal: bool = True, scal
     request are not written.  scale, out and workspace as in paged_attention."""
     idx, dt = query.get_device(), query.dtype
     code = _DT16.get(dt)
+    shape, ks = query.shape, key.shape
     a, b, c = query.stride(), key.stride(), value.stride()
-    if not (idx >= 0 and code is not None and query.dim() == 3 and key.dim() == 3 and key.shape == value.shape
-            and key.size(0) == query.size(0) and key.size(2) == query.size(2) and a[2] == b[2] == c[2] == 1
+    if not (idx >= 0 and code is not None and len(shape) == 3 and len(ks) == 3 and value.shape == ks
+            and ks[0] == shape[0] and ks[2] == shape[2] and a[2] == b[2] == c[2] == 1
             and key.dtype is dt and value.dtype is dt and key.get_device() == idx and value.get_device() == idx
             and seq_starts.dtype is _I32 and seq_starts.get_device() == idx and seq_starts.dim() == 1
             and seq_starts.is_contiguous() and seq_starts.numel() >= 1):
         _refuse_prompt(query, key, value, seq_starts)
-    T, H, D = query.shape
+    T, H, D = shape
     o = _out(query, out)
-    ws, ws_bytes = _workspace(workspace, T, H, D, query)
+    ws, ws_bytes, _keep = _workspace(workspace, idx, T, D)
     e = o.stride()
-    with _On(idx) as st:
-        _check(_L.jo_prompt_attention(
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), seq_starts.data_ptr(), o.data_ptr(), T,
-            seq_starts.numel() - 1, H, key.size(1), D, _S4(a[0], a[1], e[0], e[1]), _S4(b[0], b[1], c[0], c[1]),
-            bool(causal), 1.0 / math.sqrt(D) if scale is None else scale, code, ws.data_ptr(), ws_bytes, st))
+    _call(_L.jo_prompt_attention, idx, query.data_ptr(), key.data_ptr(), value.data_ptr(), seq_starts.data_ptr(),
+          o.data_ptr(), T, seq_starts.numel() - 1, H, ks[1], D, _S4(a[0], a[1], e[0], e[1]),
+          _S4(b[0], b[1], c[0], c[1]), bool(causal), 1.0 / math.sqrt(D) if scale is None else scale, code, ws, ws_bytes)
     return o
 
 

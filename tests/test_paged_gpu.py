@@ -435,7 +435,7 @@ def test_other_stream_and_graph(jo, cuda):
     k, v = (torch.randn(N, Hk, D, device=cuda).to(torch.bfloat16) for _ in "kv")
     lay = jo.PagedLayout.empty(B, N, cuda)
     out = torch.zeros_like(q)
-    ws = torch.empty(jo.varlen_attention_workspace(N, H, D), dtype=torch.uint8, device=cuda)
+    ws = torch.empty(jo.varlen_attention_workspace(12 * page, D), dtype=torch.uint8, device=cuda)
 
     def step():
         jo.paged_layout(cached, new, table, free, page, N, out=lay)
