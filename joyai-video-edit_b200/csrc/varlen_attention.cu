@@ -22,6 +22,12 @@
 //                would turn a NaN there into NaN), and a value row that only some
 //                rows may see is searched for NaN and infinities
 //   warp 11      walks the block's range and hands its pieces to the others
+//
+// PAIR: two blocks (a cluster) take an item of 512 rows together, tile t of the
+// one above tile t of the other in one cta_group::2 MMA of 256 rows.  Each block
+// loads half of K's keys and half of V's columns, so the shared memory that an MMA
+// reads besides its own 128 rows, what bounds it in the single form, is halved, and
+// twice as many steps are in flight.  The even block issues the MMAs.
 //   warps 0-7    softmax: one thread per row, P over S in tensor memory
 // The running maximum only moves when it grows by more than 2^8, so most steps
 // leave O alone.
@@ -35,6 +41,8 @@ namespace vattn {
 constexpr int kRows = 128;               // rows of a tile
 constexpr int kKeys = 128;               // keys of a step
 constexpr int kThreads = 384;
+// Rows of a request from which blocks work in pairs.
+constexpr int kPairRows = 2048;
 constexpr int kLead = 2;                 // steps that an item's beginning and end cost
 constexpr int kMin = 3;                  // steps of the shortest piece
 using Steps = Work<kKeys, kLead, kMin>;
@@ -59,19 +67,23 @@ struct Task {
   int pad[3];
 };
 
-template <int D> struct Cfg {
+template <int D, bool PAIR> struct Cfg {
+  static constexpr int N = PAIR ? 2 : 1;                     // blocks of an item
   static constexpr int HALVES = D / 64;
-  static constexpr int HALF = kKeys * 128;                   // 128 rows x 64 elements
-  static constexpr int TILE = HALVES * HALF;
-  static constexpr int ST = D == 128 ? 2 : 4;                // K and V steps in flight
-  static constexpr int K0 = 2 * TILE, V0 = K0 + ST * TILE;
-  static constexpr int OUT = V0 + ST * TILE;                 // 2 KB of a softmax warp: 32 rows x 32 columns on their way out
+  static constexpr int HALF = kRows * 128;                   // 128 rows x 64 elements
+  static constexpr int TILE = HALVES * HALF;                 // Q
+  static constexpr int STAGE = TILE / N;                     // this block's part of K or V of a step
+  static constexpr int KHALF = HALF / N;                     // K: its keys x 64 elements
+  static constexpr int ST = 65536 / STAGE;                   // K and V steps in flight, 64 KB each
+  static constexpr int K0 = 2 * TILE, V0 = K0 + ST * STAGE;
+  static constexpr int OUT = V0 + ST * STAGE;                // 2 KB of a softmax warp: 32 rows x 32 columns on their way out
   static constexpr int TASKS = OUT + 8 * 2048;
   static constexpr int BARS = TASKS + kPieces * (int)sizeof(Task);
   enum : int { B_QF = 0, B_QE = 1, B_SF = 2, B_PF = 4, B_OF = 6, B_TF = 8, B_TE = B_TF + kPieces, B_KF = B_TE + kPieces,
                B_KE = B_KF + ST, B_VF = B_KE + ST, B_VE = B_VF + ST, B_VG = B_VE + ST, B_END = B_VG + ST, B_N };
   static constexpr int BYTES = BARS + 512 /* barriers, flags */ + 1024 /* alignment */;
-  static_assert(B_N * 8 + 8 + 4 * ST <= 512, "");
+  static_assert(B_N * 8 + 8 + 4 * N * ST <= 512, "");
+  static_assert(!PAIR || D == 128, "");
 };
 
 struct Maps {
@@ -89,8 +101,9 @@ __device__ __forceinline__ int task_visible(const Params& p, const Task& t, int 
 
 // O (+)= P V for one row on the CUDA cores: the step's V holds a NaN or an
 // infinity that this row may not see, and a matrix product would spread it.
+// v0, v1: cluster addresses of the step's V, columns 0-63 and 64-127.
 template <typename T, int D>
-__device__ __noinline__ void careful_pv(uint32_t tP, uint32_t tO, const unsigned char* v, bool first, int lim) {
+__device__ __noinline__ void careful_pv(uint32_t tP, uint32_t tO, uint32_t v0, uint32_t v1, bool first, int lim) {
 #pragma unroll 1
   for (int c = 0; c < D; c += 32) {
     uint32_t o[32];
@@ -116,7 +129,7 @@ __device__ __noinline__ void careful_pv(uint32_t tP, uint32_t tO, const unsigned
         const bool seen = k + kk < lim;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint4 x = *reinterpret_cast<const uint4*>(v + swizzled(k + kk, c + 8 * i, Cfg<D>::HALF));
+          const uint4 x = ld_cluster((c < 64 ? v0 : v1) + swizzled(k + kk, (c & 63) + 8 * i, 0));
           const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -135,10 +148,10 @@ __device__ __noinline__ void careful_pv(uint32_t tP, uint32_t tO, const unsigned
   tmem_wait_st();
 }
 
-template <typename T, int D>
+template <typename T, int D, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ Maps maps, const Params p) {
-  using C = Cfg<D>;
-  constexpr int ST = C::ST;
+  using C = Cfg<D, PAIR>;
+  constexpr int ST = C::ST, N = C::N;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ Steps::Scan<kThreads / 32> scan;
   __shared__ Steps::Near near;
@@ -148,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::B_N);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* vflag = abort_flag + 1;  // [ST]: a NaN or infinity found in an edge step's V
+  volatile int* vflag = abort_flag + 1;  // [ST][N]: a NaN or infinity found in an edge step's V, by each block's guard
   const uint32_t bar0 = smem_u32(bars);
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
 #define WAIT(i, parity, code) mbar_wait(BAR(i), (parity), abort_flag, &g_fault, (code))
@@ -157,6 +170,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #define TASK(n) (tasks[(n) % kPieces])
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const int unit = blockIdx.x / N;       // the block or pair among its like
   const Request early = (int)threadIdx.x < p.batch ? request(p, threadIdx.x) : Request{0, 0, 0};
   launch_dependents();
   if (threadIdx.x == 0) {
@@ -165,19 +180,19 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     mbar_init(BAR(C::B_END), 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(BAR(C::B_SF + t), 1);
-      mbar_init(BAR(C::B_PF + t), 4);    // one arrival per softmax warp
+      mbar_init(BAR(C::B_PF + t), 4 * N);          // one arrival per softmax warp (on the even block's)
       mbar_init(BAR(C::B_OF + t), 1);
     }
     for (int s = 0; s < kPieces; ++s) {
       mbar_init(BAR(C::B_TF + s), 1);
-      mbar_init(BAR(C::B_TE + s), 11);   // every warp but the one that hands them out
+      mbar_init(BAR(C::B_TE + s), rank == 0 ? 11 : 10);   // every warp but the one that hands them out; one issues MMAs
     }
     for (int s = 0; s < ST; ++s) {
       mbar_init(BAR(C::B_KF + s), 1);
       mbar_init(BAR(C::B_KE + s), 1);
       mbar_init(BAR(C::B_VF + s), 1);
       mbar_init(BAR(C::B_VE + s), 1);
-      mbar_init(BAR(C::B_VG + s), 1);
+      mbar_init(BAR(C::B_VG + s), N);              // one per guard
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -188,20 +203,22 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     tma_prefetch_map(&maps.k);
     tma_prefetch_map(&maps.v);
   }
-  if (warp == 9) tmem_alloc_512(smem_u32(tmem_slot));
+  if (warp == 9) tmem_alloc_512<PAIR>(smem_u32(tmem_slot));
   Range range;
-  Steps::find<kThreads / 32>(p, early, 2 * maps.tpt, blockIdx.x, gridDim.x, scan, near, range);
+  Steps::find<kThreads / 32>(p, early, 2 * N * maps.tpt, unit, gridDim.x / N, scan, near, range);
   fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync(); else __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t sq = smem_u32(smem), sk = sq + C::K0, sv = sq + C::V0;
   const int tpt = maps.tpt;
+  // place `bar` in the even block
+  auto even = [&](uint32_t bar) { return PAIR ? map_to_rank(bar, 0) : bar; };
 
   if (warp == 11) {
     // ------------------------------------------------------ hands out pieces --
     if (lane == 0) {
-      Walk walk(p, 2 * tpt, near, range);
+      Walk walk(p, 2 * N * tpt, near, range);
       Piece s;
       Begun begun{0, 0, 0, 0};
       bool more = true;
@@ -215,34 +232,39 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         t.a = 0;
         t.e = -1;
         if (more) {
-          const int tok = s.i * 2 * tpt;
+          const int tok = s.i * 2 * N * tpt;
           t.a = s.a;
           t.e = s.e;
           t.tok = s.r.first + tok;
-          t.ntok = min(2 * tpt, s.r.n - tok);
+          t.ntok = min(2 * N * tpt, s.r.n - tok);
           t.before = s.r.keys - s.r.n + tok;
           t.keys = s.r.keys;
           t.kfirst = s.r.first;
           t.b = s.b;
           t.h = s.h;
           t.edge = task_visible(p, t, 0) / kKeys;
-          t.end[0] = max(s.a, min(s.e, max(1, div_up(task_visible(p, t, min(t.ntok, tpt) - 1), kKeys))));
-          t.end[1] = t.ntok > tpt ? s.e : s.a;
-          t.slot = s.whole() ? -1 : 2 * blockIdx.x + (s.a == 0);
+          t.end[0] = max(s.a, min(s.e, max(1, div_up(task_visible(p, t, min(t.ntok, N * tpt) - 1), kKeys))));
+          t.end[1] = t.ntok > N * tpt ? s.e : s.a;
+          t.slot = s.whole() ? -1 : 2 * unit + (s.a == 0 ? 1 : 0);
           if (s.a == 0 && s.e < s.steps)       // only the last piece ends inside an item
-            begun = Begun{Steps::later_blocks(range, s, blockIdx.x), t.tok, t.ntok, t.h};
+            begun = Begun{Steps::later_blocks(range, s, unit), t.tok, t.ntok, t.h};
         }
         TASK(n) = t;
         mbar_arrive(BAR(C::B_TF + n % kPieces));
       }
-      if (maps.begun) maps.begun[blockIdx.x] = begun;
+      if (maps.begun && rank == 0) maps.begun[unit] = begun;
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------- producer --
-    const int boxes = kKeys / maps.box;
-    const int bx = lane % boxes, half = lane / boxes;         // this lane's copy of a step
-    const bool mine = lane < boxes * C::HALVES;
-    const uint32_t dst = half * C::HALF + bx * maps.box * 128;
+    // This lane's copies of a step: `box` keys x 64 columns of K and of V each.
+    // A pair's block has half of K's keys and half of V's columns.
+    const int copies = kKeys / maps.box * C::HALVES / N;
+    const bool mine = lane < copies;
+    const int k_boxes = kKeys / N / maps.box, v_boxes = kKeys / maps.box;
+    const int kb = lane % k_boxes, kh = lane / k_boxes, vb = lane % v_boxes, vh = lane / v_boxes;
+    const int k_key = rank * (kKeys / 2) + kb * maps.box, v_key = vb * maps.box;
+    const uint32_t k_dst = kh * C::KHALF + kb * maps.box * 128, v_dst = vh * C::HALF + vb * maps.box * 128;
+    const int k_col = kh * 64, v_col = (PAIR ? rank : vh) * 64;
     uint32_t it = 0, v_issued = 0, n = 0;
     for (;; ++n) {
       if (!__all_sync(0xffffffffu, NEXT_TASK(n))) break;
@@ -262,27 +284,34 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           w0 = w1;
           kv_place(p, t.kfirst, t.keys, t.b, (j + 4) * kKeys + lane * 16, z1, w1);
         }
-        const int from = ahead * 8 + bx * (maps.box / 16);
-        const int z = __shfl_sync(0xffffffffu, z0, from), w = __shfl_sync(0xffffffffu, w0, from);
+        const int k_from = (ahead * 8 + k_key / 16) & 31, v_from = (ahead * 8 + v_key / 16) & 31;
+        const int kz = __shfl_sync(0xffffffffu, z0, k_from), kw = __shfl_sync(0xffffffffu, w0, k_from);
+        const int vz = __shfl_sync(0xffffffffu, z0, v_from), vw = __shfl_sync(0xffffffffu, w0, v_from);
         const int st = it % ST;
         const uint32_t ph = (it / ST) & 1;
         ok = __all_sync(0xffffffffu, WAIT(C::B_KE + st, ph ^ 1, 1));
         if (!ok) break;
-        if (lane == 0) mbar_expect_tx(BAR(C::B_KF + st), C::TILE);
+        // K's and Q's completion is counted on the even block's barriers, for both
+        if (lane == 0 && rank == 0) mbar_expect_tx(BAR(C::B_KF + st), N * C::STAGE);
         __syncwarp();
-        if (mine) tma_load_4d(sk + st * C::TILE + dst, &maps.k, half * 64, t.h, z, w, BAR(C::B_KF + st));
+        if (mine) {
+          if (PAIR) tma_load_4d_pair(sk + st * C::STAGE + k_dst, &maps.k, k_col, t.h, kz, kw, even(BAR(C::B_KF + st)));
+          else tma_load_4d(sk + st * C::STAGE + k_dst, &maps.k, k_col, t.h, kz, kw, BAR(C::B_KF + st));
+        }
         if (j == t.a) {
           ok = __all_sync(0xffffffffu, WAIT(C::B_QE, (n & 1) ^ 1, 2));
           if (!ok) {
             ++it;
             break;
           }
-          const int tiles = t.ntok > tpt ? 2 : 1;
-          if (lane == 0) mbar_expect_tx(BAR(C::B_QF), tiles * D * 2 * p.group * tpt);
+          const int tiles = t.ntok > N * tpt ? 2 : 1;
+          if (lane == 0 && rank == 0) mbar_expect_tx(BAR(C::B_QF), N * tiles * D * 2 * p.group * tpt);
           __syncwarp();
           if (lane < tiles * C::HALVES) {
-            const int tl = lane / C::HALVES, hf = lane % C::HALVES;
-            tma_load_4d(sq + tl * C::TILE + hf * C::HALF, &maps.q, hf * 64, 0, t.h, t.tok + tl * tpt, BAR(C::B_QF));
+            const int tl = lane / C::HALVES, hf = lane % C::HALVES, tok = t.tok + (tl * N + rank) * tpt;
+            const uint32_t dst = sq + tl * C::TILE + hf * C::HALF;
+            if (PAIR) tma_load_4d_pair(dst, &maps.q, hf * 64, 0, t.h, tok, even(BAR(C::B_QF)));
+            else tma_load_4d(dst, &maps.q, hf * 64, 0, t.h, tok, BAR(C::B_QF));
           }
         }
         ok = __all_sync(0xffffffffu, WAIT(C::B_VE + st, ph ^ 1, 3));
@@ -290,39 +319,40 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           ++it;
           break;
         }
-        if (lane == 0) mbar_expect_tx(BAR(C::B_VF + st), C::TILE);
+        if (lane == 0) mbar_expect_tx(BAR(C::B_VF + st), C::STAGE);
         __syncwarp();
-        if (mine) tma_load_4d(sv + st * C::TILE + dst, &maps.v, half * 64, t.h, z, w, BAR(C::B_VF + st));
+        if (mine) tma_load_4d(sv + st * C::STAGE + v_dst, &maps.v, v_col, t.h, vz, vw, BAR(C::B_VF + st));
         v_issued = it + 1;
       }
       if (!ok) break;
     }
-    // Every copy issued lands before the block leaves.
+    // Every copy issued lands before the block leaves.  (An odd block sees those of
+    // K and Q by their use; a wait that gave up is two seconds past them.)
     if (lane == 0) {
-      for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i) mbar_drain(BAR(C::B_KF + i % ST), (i / ST) & 1);
+      const int kbar = rank == 0 ? C::B_KF : C::B_KE;
+      for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i) mbar_drain(BAR(kbar + i % ST), (i / ST) & 1);
       for (uint32_t i = v_issued > ST ? v_issued - ST : 0; i < v_issued; ++i)
         mbar_drain(BAR(C::B_VF + i % ST), (i / ST) & 1);
-      if (n) mbar_drain(BAR(C::B_QF), (n - 1) & 1);
+      if (n) mbar_drain(BAR(rank == 0 ? C::B_QF : C::B_QE), (n - 1) & 1);
     }
   } else if (warp == 9) {
     // ----------------------------------------------------------- MMA issuer --
-    if (lane == 0) {
-      const uint32_t ID_QK = instr_desc<T>(kRows, kKeys, false) | (p.negate ? 1u << 13 : 0u);   // bit 13: -A
-      constexpr uint32_t ID_PV = instr_desc<T>(kRows, D, true);
+    if (lane == 0 && rank == 0) {
+      const uint32_t ID_QK = instr_desc<T>(N * kRows, kKeys, false) | (p.negate ? 1u << 13 : 0u);   // bit 13: -A
+      constexpr uint32_t ID_PV = instr_desc<T>(N * kRows, D, true);
       auto qk = [&](int t, int st) {     // S_t = Q_t K^T
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * C::HALF + (kk & 3) * 32;
-          mma_ss(tmem + 256 + 128 * t, smem_desc(sq + t * C::TILE + off, 16), smem_desc(sk + st * C::TILE + off, 16),
-                 ID_QK, kk != 0);
+          mma_ss<PAIR>(tmem + 256 + 128 * t, smem_desc(sq + t * C::TILE + (kk >> 2) * C::HALF + (kk & 3) * 32, 16),
+                       smem_desc(sk + st * C::STAGE + (kk >> 2) * C::KHALF + (kk & 3) * 32, 16), ID_QK, kk != 0);
         }
-        mma_commit(BAR(C::B_SF + t));
+        mma_commit<PAIR>(BAR(C::B_SF + t));
       };
       auto pv = [&](int t, int st, bool acc) {   // O_t (+)= P_t V
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
-          mma_ts(tmem + 128 * t, tmem + 256 + 128 * t + kk * 8, smem_desc(sv + st * C::TILE + kk * 2048, C::HALF),
-                 ID_PV, (acc || kk != 0) ? 1u : 0u);
+          mma_ts<PAIR>(tmem + 128 * t, tmem + 256 + 128 * t + kk * 8, smem_desc(sv + st * C::STAGE + kk * 2048, C::HALF),
+                       ID_PV, (acc || kk != 0) ? 1u : 0u);
       };
       uint32_t it = 0, n = 0, seen[2] = {0, 0};
       uint32_t guarded = 0;              // parity of each place's guarded steps
@@ -341,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           fence_after();
           for (int t = 0; t < 2; ++t)
             if (j < end[t]) qk(t, 0);
-          mma_commit(BAR(C::B_KE));
-          if (j + 1 == e) mma_commit(BAR(C::B_QE));
+          mma_commit<PAIR>(BAR(C::B_KE));
+          if (j + 1 == e) mma_commit<PAIR>(BAR(C::B_QE));
         }
       }
       while (more && ok) {
@@ -361,7 +391,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
         const int st = it % ST, nst = (it + 1) % ST;
         bool careful = false;
-        if (j < edge) {
+        if (PAIR) {                      // both guards report every step: V's halves complete on their own blocks' barriers
+          if (!WAIT(C::B_VG + st, (it / ST) & 1, 15)) break;
+          if (j >= edge) {
+            fence_acquire_cluster();
+            careful = vflag[st * N] | vflag[st * N + N - 1];
+          }
+        } else if (j < edge) {
           if (!WAIT(C::B_VF + st, (it / ST) & 1, 6)) break;
         } else {
           if (!WAIT(C::B_VG + st, (guarded >> st) & 1, 15)) break;
@@ -376,9 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             ++seen[t];
             fence_after();
             if (!careful) pv(t, st, j > a);
-            if (j + 1 == end[t]) mma_commit(BAR(C::B_OF + t));
+            if (j + 1 == end[t]) mma_commit<PAIR>(BAR(C::B_OF + t));
           }
-          if (t == 1) mma_commit(BAR(C::B_VE + st));
+          if (t == 1) mma_commit<PAIR>(BAR(C::B_VE + st));
           if (more && nj < nend[t]) {
             if (!waited) {
               ok = (!turn || WAIT(C::B_QF, n & 1, 9)) && WAIT(C::B_KF + nst, ((it + 1) / ST) & 1, 10);
@@ -391,14 +427,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
         if (!ok) break;
         if (more) {
-          mma_commit(BAR(C::B_KE + nst));
-          if (nj + 1 == ne) mma_commit(BAR(C::B_QE));
+          mma_commit<PAIR>(BAR(C::B_KE + nst));
+          if (nj + 1 == ne) mma_commit<PAIR>(BAR(C::B_QE));
         }
         a = na, e = ne, j = nj, end[0] = nend[0], end[1] = nend[1], edge = nedge;
         ++it;
       }
       // Every MMA issued completes before tensor memory is freed.
-      mma_commit(BAR(C::B_END));
+      mma_commit<PAIR>(BAR(C::B_END));
       mbar_drain(BAR(C::B_END), 0);
     }
   } else if (warp == 10) {
@@ -416,36 +452,56 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         const int st = it % ST;
         ok = __all_sync(0xffffffffu, WAIT(C::B_VF + st, (it / ST) & 1, 11));
         if (!ok) break;
-        if (j < t.edge) continue;
-        // Rows lo.. are searched (a few more below them do no harm), rows hi.. zeroed.
-        // Eight rows at a time, all loads before their use: at one load at a time
-        // this took four steps' time.
-        const int lo = max(0, some - j * kKeys), hi = min(kKeys, max(0, most - j * kKeys));
-        constexpr int CH = D / 8, STEP = 32 / CH;      // 16-byte vectors of a row; rows of one load of the warp
-        const int col = lane % CH, row0 = lane / CH;
-        unsigned char* v = smem + C::V0 + st * C::TILE + (col >> 3) * C::HALF;
-        uint32_t top = 0;
-        for (int r8 = lo & ~7; r8 < kKeys; r8 += 8) {
-          uint4 y[8 / STEP];
+        int bad = 0;
+        if (j >= t.edge) {
+          // Rows lo.. are searched (a few more below them do no harm), rows hi.. zeroed.
+          // Eight rows at a time, all loads before their use: at one load at a time
+          // this took four steps' time.
+          const int lo = max(0, some - j * kKeys), hi = min(kKeys, max(0, most - j * kKeys));
+          constexpr int CH = D / N / 8, STEP = 32 / CH;      // 16-byte vectors of a row here; rows of one load of the warp
+          const int col = lane % CH, row0 = lane / CH;
+          unsigned char* v = smem + C::V0 + st * C::STAGE + (col >> 3) * C::HALF;
+          uint32_t top[4] = {0, 0, 0, 0};
+          for (int r8 = lo & ~7; r8 < kKeys; r8 += 8) {
+            uint4 y[8 / STEP];
 #pragma unroll
-          for (int k = 0; k < 8 / STEP; ++k) {
-            const int r = k * STEP + row0;             // row & 7
-            uint4* x = reinterpret_cast<uint4*>(v + (r8 + r) * 128 + (((col & 7) ^ r) << 4));
-            if (r8 + r < hi) {
-              y[k] = *x;
-            } else {
-              y[k] = make_uint4(0, 0, 0, 0);
-              *x = y[k];
+            for (int k = 0; k < 8 / STEP; ++k) {
+              const int r = k * STEP + row0;                 // row & 7
+              uint4* x = reinterpret_cast<uint4*>(v + (r8 + r) * 128 + (((col & 7) ^ r) << 4));
+              if (r8 + r < hi) {
+                y[k] = *x;
+              } else {
+                y[k] = make_uint4(0, 0, 0, 0);
+                *x = y[k];
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 8 / STEP; ++k) {
+              top[0] = absmax2(top[0], y[k].x);
+              top[1] = absmax2(top[1], y[k].y);
+              top[2] = absmax2(top[2], y[k].z);
+              top[3] = absmax2(top[3], y[k].w);
             }
           }
-#pragma unroll
-          for (int k = 0; k < 8 / STEP; ++k)
-            top = absmax2(absmax2(absmax2(absmax2(top, y[k].x), y[k].y), y[k].z), y[k].w);
+          bad = absmax2_fold(absmax2(absmax2(top[0], top[1]), absmax2(top[2], top[3]))) >= Bits16<T>::kInf;
+          fence_async_smem();
+          bad = __any_sync(0xffffffffu, bad);
+        } else if (!PAIR) {
+          continue;
         }
-        int bad = absmax2_fold(top) >= Bits16<T>::kInf;
-        fence_async_smem();
-        bad = __any_sync(0xffffffffu, bad);
-        if (lane == 0) {
+        if (PAIR) {
+          // to both blocks: lane r tells block r
+          if (lane < N) {
+            const uint32_t bar = map_to_rank(BAR(C::B_VG + st), lane);
+            if (j >= t.edge) {
+              st_cluster(map_to_rank(smem_u32(const_cast<int*>(vflag + st * N)) + 4 * rank, lane), bad);
+              mbar_arrive_cluster<true>(bar);
+            } else {
+              mbar_arrive_cluster<false>(bar);
+            }
+          }
+          __syncwarp();
+        } else if (lane == 0) {
           vflag[st] = bad;
           mbar_arrive(BAR(C::B_VG + st));
         }
@@ -461,13 +517,15 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const uint32_t tO = tmem + t * 128 + lane_off;
     const float c = p.scale_log2;
     const int row_tok = row / p.group;             // of this row, in its tile
+    const int ti = t * N + rank;                   // the tile in its item
+    const uint32_t pf = even(BAR(C::B_PF + t));
     uint32_t it = 0, tiles = 0, outs = 0, guarded = 0;
     for (uint32_t n = 0;; ++n) {
       if (!__all_sync(0xffffffffu, NEXT_TASK(n))) break;
       const Task& task = TASK(n);
       if (task.e < 0) break;
       const int a = task.a, e = task.e, end = task.end[t], first = task.edge;
-      const int k_tok = t * tpt + row_tok;         // the row's token in the item
+      const int k_tok = ti * tpt + row_tok;        // the row's token in the item
       const int limit = task_visible(p, task, min(k_tok, task.ntok - 1));
       float m = kNoMax;                            // running max of s * c (may lag the true one by less than 8)
       float l = 0.f;                               // running sum
@@ -537,13 +595,20 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         tmem_wait_st();
         if (edge) {
           const int st = it % ST;
-          ok = __all_sync(0xffffffffu, WAIT(C::B_VG + st, (~guarded >> st) & 1, 13));
+          ok = __all_sync(0xffffffffu, WAIT(C::B_VG + st, PAIR ? (it / ST) & 1 : (~guarded >> st) & 1, 13));
           if (!ok) break;
-          if (vflag[st]) careful_pv<T, D>(tS, tO, smem + C::V0 + st * C::TILE, j == a, lim);
+          if (PAIR) fence_acquire_cluster();
+          if (vflag[st * N] | vflag[st * N + N - 1]) {
+            const uint32_t v = sv + st * C::STAGE;
+            careful_pv<T, D>(tS, tO, PAIR ? map_to_rank(v, 0) : v, PAIR ? map_to_rank(v, 1) : v + C::HALF, j == a, lim);
+          }
         }
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(BAR(C::B_PF + t));
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster<false>(pf);
+          else mbar_arrive(pf);
+        }
       }
       if (!ok) break;
       // ---- epilogue ----
@@ -592,8 +657,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           }
         }
       } else {
-        Slot<D, 2 * kRows>& slot = static_cast<Slot<D, 2 * kRows>*>(maps.partial)[task.slot];
-        const int r2 = t * kRows + row;
+        Slot<D, 2 * N * kRows>& slot = static_cast<Slot<D, 2 * N * kRows>*>(maps.partial)[task.slot];
+        const int r2 = ti * kRows + row;
         slot.ml[r2] = make_float2(m, l);
         if (has) {
 #pragma unroll 1
@@ -619,9 +684,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   // does not end before them.
   wait_for_primary();
   fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync(); else __syncthreads();
   fence_after();
-  if (warp == 9) tmem_free_512(tmem);
+  if (warp == 9) tmem_free_512<PAIR>(tmem);
 #undef BAR
 #undef WAIT
 #undef NEXT_TASK
@@ -677,49 +742,63 @@ static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int
   return JO_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool PAIR>
 static int launch_tiles(const char* what, const Params& p, void* workspace, bool overlap, cudaStream_t stream) {
   constexpr bool bf16 = IsBf16<T>::v;
   Maps maps;
   maps.tpt = kRows / p.group;
-  const int blocks = sm_count();
+  constexpr int N = PAIR ? 2 : 1;
+  const int units = sm_count() / N;
   const int64_t qd[4] = {D, p.group, p.kv_heads, p.tokens}, qs[3] = {p.q_hs, p.q_hs * p.group, p.q_ts};
   const int qb[4] = {64, p.group, 1, maps.tpt};
-  if (!make_map_4d(&maps.q, bf16, p.q, qd, qs, qb) || !kv_maps(p, bf16, kKeys, &maps.k, &maps.v, &maps.box)) {
+  if (!make_map_4d(&maps.q, bf16, p.q, qd, qs, qb) || !kv_maps(p, bf16, kKeys / N, &maps.k, &maps.v, &maps.box)) {
     set_error("%s: cuTensorMapEncodeTiled failed", what);
     return JO_ERR_CUDA;
   }
   const bool split = tiles_split(max_keys(p));
   maps.begun = split ? static_cast<Begun*>(workspace) : nullptr;
-  maps.partial = static_cast<char*>(workspace) + begun_bytes(blocks);
+  maps.partial = static_cast<char*>(workspace) + begun_bytes(sm_count());
   static bool attr[kMaxDevices] = {};
   const int dev = device_slot();
   if (!attr[dev]) {
-    if (cudaFuncSetAttribute(tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::BYTES) != cudaSuccess)
+    if (cudaFuncSetAttribute(tile_kernel<T, D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, PAIR>::BYTES) != cudaSuccess)
       return check_launch(what);
     attr[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.gridDim = dim3((unsigned)(units * N));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<D>::BYTES;
+  cfg.dynamicSmemBytes = Cfg<D, PAIR>::BYTES;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute at[2];
   cfg.attrs = at;
-  cfg.numAttrs = overlap ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, tile_kernel<T, D>, maps, p) != cudaSuccess) return check_launch(what);
-  if (split) launch_join<T, D, 2 * kRows, kRows, 1>(p, maps.partial, maps.begun, maps.tpt, blocks, stream);
+  cfg.numAttrs = 0;
+  if (overlap) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (PAIR) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = 2;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (cudaLaunchKernelEx(&cfg, tile_kernel<T, D, PAIR>, maps, p) != cudaSuccess) return check_launch(what);
+  if (split) launch_join<T, D, 2 * N * kRows, kRows, 1, 8>(p, maps.partial, maps.begun, maps.tpt, units, stream);
   return check_launch(what);
 }
 
-static int launch_all_tiles(const char* what, const Params& p, int dtype, void* workspace, bool overlap, cudaStream_t s) {
-  if (dtype == JO_DTYPE_BF16)
-    return p.head_dim == 64 ? launch_tiles<__nv_bfloat16, 64>(what, p, workspace, overlap, s)
-                            : launch_tiles<__nv_bfloat16, 128>(what, p, workspace, overlap, s);
-  return p.head_dim == 64 ? launch_tiles<__half, 64>(what, p, workspace, overlap, s)
-                          : launch_tiles<__half, 128>(what, p, workspace, overlap, s);
+// rows: those of a typical request, as far as the host knows.
+template <typename T>
+static int launch_type(const char* what, const Params& p, int64_t rows, void* workspace, bool overlap, cudaStream_t s) {
+  if (p.head_dim == 64) return launch_tiles<T, 64, false>(what, p, workspace, overlap, s);
+  return rows >= kPairRows ? launch_tiles<T, 128, true>(what, p, workspace, overlap, s)
+                           : launch_tiles<T, 128, false>(what, p, workspace, overlap, s);
+}
+static int launch_all_tiles(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, bool overlap,
+                            cudaStream_t s) {
+  return dtype == JO_DTYPE_BF16 ? launch_type<__nv_bfloat16>(what, p, rows, workspace, overlap, s)
+                                : launch_type<__half>(what, p, rows, workspace, overlap, s);
 }
 
 static int launch(const char* what, Params& p, int64_t max_query_len, int dtype, void* workspace,
@@ -739,8 +818,10 @@ static int launch(const char* what, Params& p, int64_t max_query_len, int dtype,
   // both kinds, each kernel takes its own.
   p.min_rows = 1;
   p.max_rows = INT32_MAX;
-  if (!p.table) return launch_all_tiles(what, p, dtype, workspace, false, s);
   const int64_t longest = max_query_len < p.tokens ? (max_query_len > 1 ? max_query_len : 1) : p.tokens;
+  const int64_t mean = (p.tokens + p.batch - 1) / p.batch;
+  const int64_t rows = (longest < mean ? longest : mean) * p.group;
+  if (!p.table) return launch_all_tiles(what, p, rows, dtype, workspace, false, s);
   if (p.group <= kFewRows && longest * p.group <= kFewRows)
     return launch_few(what, p, longest * p.group, dtype, workspace, s);
   if (p.group <= kFewRows && p.batch > 1) {
@@ -751,9 +832,9 @@ static int launch(const char* what, Params& p, int64_t max_query_len, int dtype,
     p.max_rows = INT32_MAX;
     // It needs nothing of what the kernel for few rows does, and has a workspace of
     // its own: its blocks may begin as that one's end.
-    return launch_all_tiles(what, p, dtype, static_cast<char*>(workspace) + few_workspace(p.head_dim), true, s);
+    return launch_all_tiles(what, p, rows, dtype, static_cast<char*>(workspace) + few_workspace(p.head_dim), true, s);
   }
-  return launch_all_tiles(what, p, dtype, workspace, false, s);
+  return launch_all_tiles(what, p, rows, dtype, workspace, false, s);
 }
 
 }  // namespace vattn

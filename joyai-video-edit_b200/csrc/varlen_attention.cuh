@@ -382,29 +382,30 @@ __device__ __forceinline__ bool row_place(int r, int group, int tpt, int n, int&
 // item that block c of the attention kernel began and did not end.  A team of
 // TEAM warps takes 32 rows and 8 columns of it (y and the team's place in the
 // block enumerate them), each lane one row; the team's warps share out the
-// partial results and warp 0 adds theirs up.  Latency-bound: the reads of four
+// partial results and warp 0 adds theirs up.  Latency-bound: the reads of DEEP
 // partial results are in flight at a time.
-template <typename T, int D, int R, int TILE, int TEAM>
-__global__ void __launch_bounds__(256) join_kernel(const Params p, const Slot<D, R>* slots, const Begun* begun, int tpt) {
-  static_assert(8 % TEAM == 0, "");
-  __shared__ float shared[TEAM > 1 ? 8 : 1][10][32];
+template <typename T, int D, int R, int TILE, int TEAM, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) join_kernel(const Params p, const Slot<D, R>* slots, const Begun* begun, int tpt) {
+  static_assert(WARPS % TEAM == 0, "");
+  __shared__ float shared[TEAM > 1 ? WARPS : 1][10][32];
   wait_for_primary();
   const int c = blockIdx.x;
   const Begun me = begun[c];
   if (me.later == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp % TEAM;
-  const int w = blockIdx.y * (8 / TEAM) + warp / TEAM;
+  const int w = blockIdx.y * (WARPS / TEAM) + warp / TEAM;
   const int col = (w % (D / 8)) * 8, r = (w / (D / 8)) * 32 + lane;
   int tok, head;
   const bool valid = row_place<TILE>(r, p.group, tpt, me.n, tok, head);
   float m = kNoMax, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int count = me.later + 1;        // slots 2c+1, 2c+2, 2c+4, ..., 2(c+later)
   const int per = (count + TEAM - 1) / TEAM, lo = member * per, hi = min(count, lo + per);
-  for (int i0 = lo; i0 < hi; i0 += 4) {
-    float2 ml[4];
-    float4 x[4], y[4];
+  constexpr int DEEP = 4;
+  for (int i0 = lo; i0 < hi; i0 += DEEP) {
+    float2 ml[DEEP];
+    float4 x[DEEP], y[DEEP];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < DEEP; ++k) {
       const int i = min(i0 + k, hi - 1);
       const Slot<D, R>& s = slots[i == 0 ? 2 * c + 1 : 2 * (c + i)];
       ml[k] = s.ml[r];
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, const Slot<D,
       y[k] = *reinterpret_cast<const float4*>(s.o[col / 4 + 1][r]);
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < DEEP; ++k) {
       if (i0 + k >= hi || ml[k].y == 0.f) continue;      // a row without a visible key there has no O either
       const float mn = fmaxf(m, ml[k].x), a = ex2(m - mn), b = ex2(ml[k].x - mn);
       m = mn;
@@ -451,18 +452,18 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, const Slot<D,
                             (int64_t)(me.h * p.group + head) * p.o_hs + col) = out;
 }
 
-template <typename T, int D, int R, int TILE, int TEAM>
+template <typename T, int D, int R, int TILE, int TEAM, int WARPS>
 inline void launch_join(const Params& p, const void* slots, const Begun* begun, int tpt, int blocks, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, R / 32 * (D / 8) / (8 / TEAM));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)blocks, R / 32 * (D / 8) / (WARPS / TEAM));
+  cfg.blockDim = dim3(32 * WARPS);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, join_kernel<T, D, R, TILE, TEAM>, p, static_cast<const Slot<D, R>*>(slots), begun, tpt);
+  cudaLaunchKernelEx(&cfg, join_kernel<T, D, R, TILE, TEAM, WARPS>, p, static_cast<const Slot<D, R>*>(slots), begun, tpt);
 }
 
 // ----------------------------------------------------------- K and V maps ----

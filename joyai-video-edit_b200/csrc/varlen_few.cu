@@ -445,7 +445,7 @@ static int launch(const char* what, const Params& p, void* workspace, cudaStream
     attr[dev] = true;
   }
   few_kernel<T, D, MT><<<blocks, kThreads, C::BYTES, stream>>>(maps, p);
-  if (split) launch_join<T, D, 32, C::R, 2>(p, maps.partial, maps.begun, maps.tpi, blocks, stream);
+  if (split) launch_join<T, D, 32, C::R, 2, 8>(p, maps.partial, maps.begun, maps.tpi, blocks, stream);
   return check_launch(what);
 }
 

@@ -539,3 +539,44 @@ def test_prefill_then_decode_equals_the_whole_prompt(jo, cuda):
         check_rows(got, ref[a:], err[a:])
         check_rows(whole[a:a + n], ref[a:], err[a:])
         a += n
+
+
+def test_more_pieces_than_are_handed_out_ahead(jo, cuda):
+    """Several long requests with many key heads: every block goes through a dozen items and more."""
+    for H, Hk, lens in ((64, 32, [1100, 1300, 1024]), (32, 32, [2100, 2300])):
+        g = torch.Generator(device=cuda).manual_seed(H)
+        T = sum(lens)
+        q = torch.randn(T, H, 128, generator=g, device=cuda).to(torch.bfloat16)
+        k, v = (torch.randn(T, Hk, 128, generator=g, device=cuda).to(torch.bfloat16) for _ in "kv")
+        got = jo.prompt_attention(q, k, v, starts_of(lens, cuda))
+        jo.check_gemm_fault()
+        a = 0
+        for n in lens:
+            check_rows(got[a:a + n], *reference(q[a:a + n], k[a:a + n], v[a:a + n], True, 1 / math.sqrt(128)))
+            a += n
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("H,Hk,new,cached,page", [
+    (16, 2, [513, 300], [100, 7], 16), (8, 1, [511, 512, 257], [0, 130, 64], 48), (12, 2, [700], [1000], 64),
+    (2, 2, [2049, 2500], [0, 300], 128), (40, 4, [400, 1, 0, 640], [30, 5, 9, 0], 32),
+])
+def test_long_chunks(jo, cuda, H, Hk, new, cached, page, dt):
+    """Requests of thousands of rows (tokens times heads of a group)."""
+    for causal in (True, False):
+        c = Case(cuda, cached, new, H, Hk, 128, page, dt, seed=H)
+        c.check(c.run(jo, causal, max_query_len=max(new)), causal)
+        jo.check_gemm_fault()
+
+
+def test_nan_in_later_tokens_of_long_chunks_stays_there(jo, cuda):
+    c = Case(cuda, [70], [900], 12, 4, 128, 16, seed=21)
+    for j, bad, col in ((70 + 300, NAN, 5), (70 + 611, math.inf, 100), (70 + 877, -math.inf, 127)):
+        c.vc[c.table[0, j // 16].item(), j % 16, :, col] = bad
+    got = c.run(jo)
+    ref, err = reference(c.q, c.ks[0], c.vs[0], True, c.scale)
+    check_rows(got[:300], ref[:300], err[:300])
+    for a, b, cols in ((300, 611, [5]), (611, 877, [5, 100]), (877, 900, [5, 100, 127])):
+        clean = [i for i in range(128) if i not in cols]
+        check_rows(got[a:b, :, clean], ref[a:b, :, clean], err[a:b, :, clean])
+        assert not torch.isfinite(got[a + 1:b, :, cols]).any()
