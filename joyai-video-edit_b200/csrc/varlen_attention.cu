@@ -41,8 +41,13 @@ namespace vattn {
 constexpr int kRows = 128;               // rows of a tile
 constexpr int kKeys = 128;               // keys of a step
 constexpr int kThreads = 384;
-// Rows of a request from which blocks work in pairs.
+// Blocks work in pairs where requests have this many rows and K and V are larger
+// than L2 by half.  Pairs halve the reads of K and V and have twice the steps in
+// flight, but wait for each other: at 11042 tokens over 32102 keys the single form
+// has 1.00-1.08 PFLOP/s with 10 heads (K and V 164 MB), pairs 1.00; with 20 heads
+// (329 MB) 0.85 and 0.94.
 constexpr int kPairRows = 2048;
+constexpr int64_t kPairBytes = 192LL << 20;
 constexpr int kLead = 2;                 // steps that an item's beginning and end cost
 constexpr int kMin = 3;                  // steps of the shortest piece
 using Steps = Work<kKeys, kLead, kMin>;
@@ -680,9 +685,6 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     }
   }
 
-  // Where this kernel began before the ones ahead of it had ended (see launch), it
-  // does not end before them.
-  wait_for_primary();
   fence_before();
   if (PAIR) cluster_sync(); else __syncthreads();
   fence_after();
@@ -691,6 +693,33 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #undef WAIT
 #undef NEXT_TASK
 #undef TASK
+}
+
+// Joins what the tile kernel (items of TR rows) and the one for few rows (items of
+// FR) left, in one launch.
+template <typename T, int D, int TR, int FR>
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p, const ToJoin tiles, const ToJoin few) {
+  __shared__ float shared[kJoinWarps][10][32];
+  wait_for_primary();
+  const int c = blockIdx.x, y = blockIdx.y;
+  if (c < tiles.blocks) {
+    if (y < join_y(D, TR, 1)) join_item<T, D, TR, kRows, 1>(p, tiles, c, y, shared);
+  } else if (y < join_y(D, 32, 2)) {
+    join_item<T, D, 32, FR, 2>(p, few, c - tiles.blocks, y, shared);
+  }
+}
+template <typename T, int D, int TR, int FR>
+static void launch_join(const Params& p, const ToJoin& tiles, const ToJoin& few, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles.blocks + few.blocks), tiles.blocks ? join_y(D, TR, 1) : join_y(D, 32, 2));
+  cfg.blockDim = dim3(32 * kJoinWarps);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, join_kernel<T, D, TR, FR>, p, tiles, few);
 }
 
 // ------------------------------------------------------------------- host --
@@ -706,6 +735,15 @@ static int64_t workspace_bytes_for(int64_t max_keys, int head_dim) {
   return tiles_split(max_keys) || few_splits(max_keys) ? tile_workspace(head_dim) + few_workspace(head_dim) : 0;
 }
 static int64_t max_keys(const Params& p) { return p.table ? (int64_t)p.width * p.page : p.tokens; }
+// The most K and V that a call can read.
+static int64_t kv_bytes(const Params& p) {
+  int64_t keys = p.tokens;
+  if (p.table) {
+    const int64_t held = (int64_t)p.num_blocks * p.page, named = p.batch * max_keys(p);
+    keys = held < named ? held : named;
+  }
+  return keys * p.kv_heads * p.head_dim * 4;
+}
 
 static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
                  int64_t head_dim, float scale, int dtype) {
@@ -743,7 +781,7 @@ static int check(const char* what, Params& p, int64_t tokens, int64_t batch, int
 }
 
 template <typename T, int D, bool PAIR>
-static int launch_tiles(const char* what, const Params& p, void* workspace, bool overlap, cudaStream_t stream) {
+static int launch_tiles(const char* what, const Params& p, void* workspace, ToJoin* join, cudaStream_t stream) {
   constexpr bool bf16 = IsBf16<T>::v;
   Maps maps;
   maps.tpt = kRows / p.group;
@@ -770,35 +808,54 @@ static int launch_tiles(const char* what, const Params& p, void* workspace, bool
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Cfg<D, PAIR>::BYTES;
   cfg.stream = stream;
-  cudaLaunchAttribute at[2];
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 0;
-  if (overlap) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (PAIR) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    at[cfg.numAttrs].val.clusterDim.x = 2;
-    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  if (cudaLaunchKernelEx(&cfg, tile_kernel<T, D, PAIR>, maps, p) != cudaSuccess) return check_launch(what);
-  if (split) launch_join<T, D, 2 * N * kRows, kRows, 1, 8>(p, maps.partial, maps.begun, maps.tpt, units, stream);
+  cfg.numAttrs = PAIR ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, tile_kernel<T, D, PAIR>, maps, p);
+  *join = ToJoin{maps.partial, maps.begun, split ? units : 0, maps.tpt};
   return check_launch(what);
 }
 
-// rows: those of a typical request, as far as the host knows.
-template <typename T>
-static int launch_type(const char* what, const Params& p, int64_t rows, void* workspace, bool overlap, cudaStream_t s) {
-  if (p.head_dim == 64) return launch_tiles<T, 64, false>(what, p, workspace, overlap, s);
-  return rows >= kPairRows ? launch_tiles<T, 128, true>(what, p, workspace, overlap, s)
-                           : launch_tiles<T, 128, false>(what, p, workspace, overlap, s);
-}
-static int launch_all_tiles(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, bool overlap,
-                            cudaStream_t s) {
-  return dtype == JO_DTYPE_BF16 ? launch_type<__nv_bfloat16>(what, p, rows, workspace, overlap, s)
-                                : launch_type<__half>(what, p, rows, workspace, overlap, s);
+// Which kernels a call takes.
+struct Plan {
+  bool few, tiles, pair;
+};
+
+template <typename T, int D>
+static int launch_type(const char* what, Params& p, const Plan& plan, int64_t rows, int dtype, void* workspace,
+                       cudaStream_t s) {
+  ToJoin tiles{nullptr, nullptr, 0, 1}, few{nullptr, nullptr, 0, 1};
+  FewShape shape{1};
+  p.min_rows = plan.few && plan.tiles ? kFewRows + 1 : 1;
+  p.max_rows = INT32_MAX;
+  if (plan.tiles) {
+    const int st = D == 128 && plan.pair ? launch_tiles<T, D, D == 128>(what, p, workspace, &tiles, s)
+                                         : launch_tiles<T, D, false>(what, p, workspace, &tiles, s);
+    if (st != JO_OK) return st;
+  }
+  if (plan.few) {
+    // Beside the tile kernel it has requests and a workspace of its own: its blocks
+    // begin as the other's end.
+    Params q = p;
+    q.min_rows = 1;
+    if (plan.tiles) q.max_rows = kFewRows;
+    const int st = launch_few(what, q, rows, dtype, static_cast<char*>(workspace) + tile_workspace(D), plan.tiles, &few,
+                              &shape, s);
+    if (st != JO_OK) return st;
+  }
+  if (tiles.blocks + few.blocks > 0) {
+    if (shape.rows16 == 1) {
+      if (D == 128 && plan.pair) launch_join<T, D, 4 * kRows, 16>(p, tiles, few, s);
+      else launch_join<T, D, 2 * kRows, 16>(p, tiles, few, s);
+    } else {
+      if (D == 128 && plan.pair) launch_join<T, D, 4 * kRows, 32>(p, tiles, few, s);
+      else launch_join<T, D, 2 * kRows, 32>(p, tiles, few, s);
+    }
+  }
+  return check_launch(what);
 }
 
 static int launch(const char* what, Params& p, int64_t max_query_len, int dtype, void* workspace,
@@ -811,30 +868,25 @@ static int launch(const char* what, Params& p, int64_t max_query_len, int dtype,
   JO_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), JO_ERR_INVALID,
              "%s: a 16-byte aligned workspace of %lld bytes is needed (got %lld)", what, (long long)need,
              (long long)workspace_bytes);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   // A request of few rows is bound by reading its keys and is served by its own
   // kernel.  Where the longest request is one, that kernel takes them all (in
   // runs of rows, should one be longer than announced); where a batch may hold
-  // both kinds, each kernel takes its own.
-  p.min_rows = 1;
-  p.max_rows = INT32_MAX;
+  // both kinds, each kernel takes its own.  (One request: the tile kernel, if it
+  // can have more than few rows.)
   const int64_t longest = max_query_len < p.tokens ? (max_query_len > 1 ? max_query_len : 1) : p.tokens;
   const int64_t mean = (p.tokens + p.batch - 1) / p.batch;
-  const int64_t rows = (longest < mean ? longest : mean) * p.group;
-  if (!p.table) return launch_all_tiles(what, p, rows, dtype, workspace, false, s);
-  if (p.group <= kFewRows && longest * p.group <= kFewRows)
-    return launch_few(what, p, longest * p.group, dtype, workspace, s);
-  if (p.group <= kFewRows && p.batch > 1) {
-    p.max_rows = kFewRows;
-    st = launch_few(what, p, kFewRows, dtype, workspace, s);
-    if (st != JO_OK) return st;
-    p.min_rows = kFewRows + 1;
-    p.max_rows = INT32_MAX;
-    // It needs nothing of what the kernel for few rows does, and has a workspace of
-    // its own: its blocks may begin as that one's end.
-    return launch_all_tiles(what, p, rows, dtype, static_cast<char*>(workspace) + few_workspace(p.head_dim), true, s);
-  }
-  return launch_all_tiles(what, p, rows, dtype, workspace, false, s);
+  const bool only_few = p.table && p.group <= kFewRows && longest * p.group <= kFewRows;
+  Plan plan;
+  plan.few = only_few || (p.table && p.group <= kFewRows && p.batch > 1);
+  plan.tiles = !only_few;
+  plan.pair = (longest < mean ? longest : mean) * p.group >= kPairRows && kv_bytes(p) >= kPairBytes;
+  const int64_t few_rows = only_few ? longest * p.group : kFewRows;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == JO_DTYPE_BF16)
+    return p.head_dim == 64 ? launch_type<__nv_bfloat16, 64>(what, p, plan, few_rows, dtype, workspace, s)
+                            : launch_type<__nv_bfloat16, 128>(what, p, plan, few_rows, dtype, workspace, s);
+  return p.head_dim == 64 ? launch_type<__half, 64>(what, p, plan, few_rows, dtype, workspace, s)
+                          : launch_type<__half, 128>(what, p, plan, few_rows, dtype, workspace, s);
 }
 
 }  // namespace vattn

@@ -378,25 +378,34 @@ __device__ __forceinline__ bool row_place(int r, int group, int tpt, int n, int&
   return k < tpt && tok < n;
 }
 
-// Adds up the partial results of the items that cuts divide.  Block (c, y): the
-// item that block c of the attention kernel began and did not end.  A team of
-// TEAM warps takes 32 rows and 8 columns of it (y and the team's place in the
-// block enumerate them), each lane one row; the team's warps share out the
-// partial results and warp 0 adds theirs up.  Latency-bound: the reads of DEEP
-// partial results are in flight at a time.
-template <typename T, int D, int R, int TILE, int TEAM, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) join_kernel(const Params p, const Slot<D, R>* slots, const Begun* begun, int tpt) {
-  static_assert(WARPS % TEAM == 0, "");
-  __shared__ float shared[TEAM > 1 ? WARPS : 1][10][32];
-  wait_for_primary();
-  const int c = blockIdx.x;
-  const Begun me = begun[c];
+// What one attention kernel left to join.
+struct ToJoin {
+  const void* slots;
+  const Begun* begun;
+  int blocks;                            // of the attention kernel
+  int tpt;                               // tokens of a tile of rows
+};
+
+// Adds up the partial results of an item that cuts divide: the item that block c of
+// the attention kernel began and did not end.  A team of TEAM warps takes 32 rows
+// and 8 columns of it (y and the team's place in the block enumerate them), each
+// lane one row; the team's warps share out the partial results and warp 0 adds
+// theirs up.  Latency-bound: the reads of four partial results are in flight at a
+// time (six, and more or larger blocks, measured slower: 54 against 49 us for 64
+// single tokens over 54480 cached ones, most of whose blocks find nothing to do).
+constexpr int kJoinWarps = 8;
+template <typename T, int D, int R, int TILE, int TEAM>
+__device__ __forceinline__ void join_item(const Params& p, const ToJoin& j, int c, int y, float (*shared)[10][32]) {
+  static_assert(kJoinWarps % TEAM == 0, "");
+  const Slot<D, R>* slots = static_cast<const Slot<D, R>*>(j.slots);
+  const Begun me = j.begun[c];
   if (me.later == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp % TEAM;
-  const int w = blockIdx.y * (WARPS / TEAM) + warp / TEAM;
+  const int w = y * (kJoinWarps / TEAM) + warp / TEAM;
   const int col = (w % (D / 8)) * 8, r = (w / (D / 8)) * 32 + lane;
+  if (w >= R / 32 * (D / 8)) return;     // (the whole block: R / 32 * D / 8 is a multiple of its teams)
   int tok, head;
-  const bool valid = row_place<TILE>(r, p.group, tpt, me.n, tok, head);
+  const bool valid = row_place<TILE>(r, p.group, j.tpt, me.n, tok, head);
   float m = kNoMax, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int count = me.later + 1;        // slots 2c+1, 2c+2, 2c+4, ..., 2(c+later)
   const int per = (count + TEAM - 1) / TEAM, lo = member * per, hi = min(count, lo + per);
@@ -451,20 +460,8 @@ __global__ void __launch_bounds__(32 * WARPS) join_kernel(const Params p, const 
   *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)(me.first + tok) * p.o_ts +
                             (int64_t)(me.h * p.group + head) * p.o_hs + col) = out;
 }
-
-template <typename T, int D, int R, int TILE, int TEAM, int WARPS>
-inline void launch_join(const Params& p, const void* slots, const Begun* begun, int tpt, int blocks, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, R / 32 * (D / 8) / (WARPS / TEAM));
-  cfg.blockDim = dim3(32 * WARPS);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, join_kernel<T, D, R, TILE, TEAM, WARPS>, p, static_cast<const Slot<D, R>*>(slots), begun, tpt);
-}
+// Blocks along y that an item of R rows needs.
+constexpr int join_y(int D, int R, int team) { return R / 32 * (D / 8) / (kJoinWarps / team); }
 
 // ----------------------------------------------------------- K and V maps ----
 // Byte of element (row, col) of a 128-byte-swizzled tile whose 64-column blocks
@@ -509,12 +506,18 @@ __device__ __forceinline__ void kv_place(const Params& p, int first, int keys, i
   }
 }
 
-// The kernel for requests of few rows (varlen_few.cu): rows, the most of any
-// request as far as the host knows it; up to kFewRows it serves them best.
+// The kernel for requests of few rows (varlen_few.cu): `rows`, the most of any
+// request as far as the host knows; up to kFewRows it serves them best.  What is
+// to be joined comes back in *join (blocks 0: nothing).  overlap: its blocks may
+// begin as those of the kernel before it end.
 constexpr int kFewRows = 32;
+struct FewShape {
+  int rows16;                            // rows of an item / 16: 1 or 2
+};
 int64_t few_workspace(int head_dim);
-bool few_splits(int64_t max_keys);     // whether an item of so many keys can have a cut inside
-int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, cudaStream_t stream);
+bool few_splits(int64_t max_keys);       // whether an item of so many keys can have a cut inside
+int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, bool overlap, ToJoin* join,
+               FewShape* shape, cudaStream_t stream);
 int few_last_fault(int reset);
 
 }  // namespace vattn

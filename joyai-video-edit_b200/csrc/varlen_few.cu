@@ -418,6 +418,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
         }
     }
   }
+  // Where this kernel began before the ones ahead of it had ended, it does not end
+  // before them.
+  wait_for_primary();
 #undef FULL
 #undef EMPTY
 }
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
 static int64_t begun_bytes(int blocks) { return ((int64_t)blocks * (int64_t)sizeof(Begun) + 15) / 16 * 16; }
 
 template <typename T, int D, int MT>
-static int launch(const char* what, const Params& p, void* workspace, cudaStream_t stream) {
+static int launch(const char* what, const Params& p, void* workspace, bool overlap, ToJoin* join, cudaStream_t stream) {
   using C = Cfg<D, MT>;
   Maps maps;
   if (!kv_maps(p, IsBf16<T>::v, kKeys, &maps.k, &maps.v, &maps.box)) {
@@ -444,14 +447,26 @@ static int launch(const char* what, const Params& p, void* workspace, cudaStream
       return check_launch(what);
     attr[dev] = true;
   }
-  few_kernel<T, D, MT><<<blocks, kThreads, C::BYTES, stream>>>(maps, p);
-  if (split) launch_join<T, D, 32, C::R, 2, 8>(p, maps.partial, maps.begun, maps.tpi, blocks, stream);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = overlap ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, few_kernel<T, D, MT>, maps, p);
+  *join = ToJoin{maps.partial, maps.begun, split ? blocks : 0, maps.tpi};
   return check_launch(what);
 }
 
 template <typename T, int D>
-static int launch_rows(const char* what, const Params& p, int64_t rows, void* workspace, cudaStream_t stream) {
-  return rows <= 16 ? launch<T, D, 1>(what, p, workspace, stream) : launch<T, D, 2>(what, p, workspace, stream);
+static int launch_rows(const char* what, const Params& p, int mt, void* workspace, bool overlap, ToJoin* join,
+                       cudaStream_t stream) {
+  return mt == 1 ? launch<T, D, 1>(what, p, workspace, overlap, join, stream)
+                 : launch<T, D, 2>(what, p, workspace, overlap, join, stream);
 }
 
 }  // namespace few
@@ -463,12 +478,14 @@ int64_t few_workspace(int head_dim) {
   return few::begun_bytes(n) + 2 * (int64_t)n * (int64_t)(head_dim == 64 ? sizeof(Slot<64, 32>) : sizeof(Slot<128, 32>));
 }
 
-int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, cudaStream_t s) {
+int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, bool overlap, ToJoin* join,
+               FewShape* shape, cudaStream_t s) {
+  const int mt = shape->rows16 = rows <= 16 ? 1 : 2;
   if (dtype == JO_DTYPE_BF16)
-    return p.head_dim == 64 ? few::launch_rows<__nv_bfloat16, 64>(what, p, rows, workspace, s)
-                            : few::launch_rows<__nv_bfloat16, 128>(what, p, rows, workspace, s);
-  return p.head_dim == 64 ? few::launch_rows<__half, 64>(what, p, rows, workspace, s)
-                          : few::launch_rows<__half, 128>(what, p, rows, workspace, s);
+    return p.head_dim == 64 ? few::launch_rows<__nv_bfloat16, 64>(what, p, mt, workspace, overlap, join, s)
+                            : few::launch_rows<__nv_bfloat16, 128>(what, p, mt, workspace, overlap, join, s);
+  return p.head_dim == 64 ? few::launch_rows<__half, 64>(what, p, mt, workspace, overlap, join, s)
+                          : few::launch_rows<__half, 128>(what, p, mt, workspace, overlap, join, s);
 }
 
 int few_last_fault(int reset) {

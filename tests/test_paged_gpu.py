@@ -556,21 +556,31 @@ def test_more_pieces_than_are_handed_out_ahead(jo, cuda):
             a += n
 
 
+def large(Hk, page):
+    """Spare blocks and table columns that make K and V larger than L2, as far as their shapes tell."""
+    n = 210 * 2 ** 20 // (page * Hk * 128 * 4)
+    return dict(spare=n, extra_width=n)
+
+
+@pytest.mark.parametrize("big", [False, True])
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 @pytest.mark.parametrize("H,Hk,new,cached,page", [
     (16, 2, [513, 300], [100, 7], 16), (8, 1, [511, 512, 257], [0, 130, 64], 48), (12, 2, [700], [1000], 64),
-    (2, 2, [2049, 2500], [0, 300], 128), (40, 4, [400, 1, 0, 640], [30, 5, 9, 0], 32),
+    (2, 2, [2049, 2500], [0, 300], 128), (40, 4, [400, 1, 0, 640], [30, 5, 9, 0], 32), (64, 16, [600], [20000], 64),
 ])
-def test_long_chunks(jo, cuda, H, Hk, new, cached, page, dt):
+def test_long_chunks(jo, cuda, H, Hk, new, cached, page, dt, big):
     """Requests of thousands of rows (tokens times heads of a group)."""
     for causal in (True, False):
-        c = Case(cuda, cached, new, H, Hk, 128, page, dt, seed=H)
-        c.check(c.run(jo, causal, max_query_len=max(new)), causal)
+        c = Case(cuda, cached, new, H, Hk, 128, page, dt, seed=H, **(large(Hk, page) if big else {}))
+        got = c.run(jo, causal, max_query_len=max(new))
+        c.check(got, causal)
         jo.check_gemm_fault()
+        assert torch.equal(got, c.run(jo, causal, max_query_len=max(new)))
 
 
-def test_nan_in_later_tokens_of_long_chunks_stays_there(jo, cuda):
-    c = Case(cuda, [70], [900], 12, 4, 128, 16, seed=21)
+@pytest.mark.parametrize("big", [False, True])
+def test_nan_in_later_tokens_of_long_chunks_stays_there(jo, cuda, big):
+    c = Case(cuda, [70], [900], 12, 4, 128, 16, seed=21, **(large(4, 16) if big else {}))
     for j, bad, col in ((70 + 300, NAN, 5), (70 + 611, math.inf, 100), (70 + 877, -math.inf, 127)):
         c.vc[c.table[0, j // 16].item(), j % 16, :, col] = bad
     got = c.run(jo)
@@ -580,3 +590,31 @@ def test_nan_in_later_tokens_of_long_chunks_stays_there(jo, cuda):
         clean = [i for i in range(128) if i not in cols]
         check_rows(got[a:b, :, clean], ref[a:b, :, clean], err[a:b, :, clean])
         assert not torch.isfinite(got[a + 1:b, :, cols]).any()
+
+
+def test_long_prompts_with_many_key_heads(jo, cuda):
+    """K and V larger than L2."""
+    lens, H, Hk = [5000, 7300, 13], 32, 32
+    T = sum(lens)
+    g = torch.Generator(device=cuda).manual_seed(22)
+    q = torch.randn(T, H, 128, generator=g, device=cuda).to(torch.bfloat16)
+    k, v = (torch.randn(T, Hk, 128, generator=g, device=cuda).to(torch.bfloat16) for _ in "kv")
+    got = jo.prompt_attention(q, k, v, starts_of(lens, cuda))
+    jo.check_gemm_fault()
+    a = 0
+    for n in lens:
+        for h in (0, 13, 31):
+            check_rows(got[a:a + n, h:h + 1], *reference(q[a:a + n, h:h + 1], k[a:a + n, h:h + 1], v[a:a + n, h:h + 1], True,
+                                                         1 / math.sqrt(128)))
+        a += n
+
+
+@pytest.mark.parametrize("H,Hk,D", [(8, 2, 128), (14, 2, 64), (32, 32, 128)])
+def test_chunks_and_single_tokens_together(jo, cuda, H, Hk, D):
+    """One call that several kernels share: every request comes out, whoever serves it."""
+    new = [1, 300, 2, 0, 64, 1, 7, 9, 1, 33, 512, 1]
+    cached = [5000, 100, 37, 11, 0, 0, 1200, 4000, 64, 2500, 1500, 12345]
+    c = Case(cuda, cached, new, H, Hk, D, 16, seed=23)
+    for _ in range(3):
+        c.check(c.run(jo))
+    jo.check_gemm_fault()
