@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0;
   const int unit = blockIdx.x / N;       // the block or pair among its like
+  wait_for_primary();                    // launched as the kernel before it ends
   const Request early = (int)threadIdx.x < p.batch ? request(p, threadIdx.x) : Request{0, 0, 0};
   launch_dependents();
   if (threadIdx.x == 0) {
@@ -701,6 +702,7 @@ template <typename T, int D, int TR, int FR>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p, const ToJoin tiles, const ToJoin few) {
   __shared__ float shared[kJoinWarps][10][32];
   wait_for_primary();
+  launch_dependents();
   const int c = blockIdx.x, y = blockIdx.y;
   if (c < tiles.blocks) {
     if (y < join_y(D, TR, 1)) join_item<T, D, TR, kRows, 1>(p, tiles, c, y, shared);
@@ -808,12 +810,14 @@ static int launch_tiles(const char* what, const Params& p, void* workspace, ToJo
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Cfg<D, PAIR>::BYTES;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = PAIR ? 1 : 0;
+  cfg.numAttrs = PAIR ? 2 : 1;
   cudaLaunchKernelEx(&cfg, tile_kernel<T, D, PAIR>, maps, p);
   *join = ToJoin{maps.partial, maps.begun, split ? units : 0, maps.tpt};
   return check_launch(what);

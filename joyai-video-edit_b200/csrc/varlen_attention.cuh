@@ -508,15 +508,15 @@ __device__ __forceinline__ void kv_place(const Params& p, int first, int keys, i
 
 // The kernel for requests of few rows (varlen_few.cu): `rows`, the most of any
 // request as far as the host knows; up to kFewRows it serves them best.  What is
-// to be joined comes back in *join (blocks 0: nothing).  overlap: its blocks may
-// begin as those of the kernel before it end.
+// to be joined comes back in *join (blocks 0: nothing).  beside: its blocks may
+// begin as those of the kernel before it end, of which it needs nothing.
 constexpr int kFewRows = 32;
 struct FewShape {
   int rows16;                            // rows of an item / 16: 1 or 2
 };
 int64_t few_workspace(int head_dim);
 bool few_splits(int64_t max_keys);       // whether an item of so many keys can have a cut inside
-int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, bool overlap, ToJoin* join,
+int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, bool beside, ToJoin* join,
                FewShape* shape, cudaStream_t stream);
 int few_last_fault(int reset);
 

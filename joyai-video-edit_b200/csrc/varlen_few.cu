@@ -50,6 +50,7 @@ struct Maps {
   CUtensorMap k, v;
   int box;                               // keys of one copy
   int tpi;                               // tokens of an item
+  int beside;                            // runs beside the kernel before it, and needs nothing of it
   void* partial;
   Begun* begun;
 };
@@ -103,6 +104,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
 #define FULL(s) (bar0 + 8u * (uint32_t)(s))
 #define EMPTY(s) (bar0 + 8u * (uint32_t)(ST + (s)))
 
+  if (!maps.beside) wait_for_primary();
   const Request early = (int)threadIdx.x < p.batch ? request(p, threadIdx.x) : Request{0, 0, 0};
   launch_dependents();
   if (threadIdx.x == 0) {
@@ -418,9 +420,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
         }
     }
   }
-  // Where this kernel began before the ones ahead of it had ended, it does not end
-  // before them.
-  wait_for_primary();
+  if (maps.beside) wait_for_primary();   // it does not end before the kernels ahead of it
 #undef FULL
 #undef EMPTY
 }
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
 static int64_t begun_bytes(int blocks) { return ((int64_t)blocks * (int64_t)sizeof(Begun) + 15) / 16 * 16; }
 
 template <typename T, int D, int MT>
-static int launch(const char* what, const Params& p, void* workspace, bool overlap, ToJoin* join, cudaStream_t stream) {
+static int launch(const char* what, const Params& p, void* workspace, bool beside, ToJoin* join, cudaStream_t stream) {
   using C = Cfg<D, MT>;
   Maps maps;
   if (!kv_maps(p, IsBf16<T>::v, kKeys, &maps.k, &maps.v, &maps.box)) {
@@ -437,6 +437,7 @@ static int launch(const char* what, const Params& p, void* workspace, bool overl
   }
   const int blocks = kBlocksPerSm * sm_count();
   maps.tpi = C::R / p.group;
+  maps.beside = beside;
   const bool split = few_splits((int64_t)p.width * p.page);
   maps.begun = split ? static_cast<Begun*>(workspace) : nullptr;
   maps.partial = static_cast<char*>(workspace) + begun_bytes(blocks);
@@ -456,17 +457,17 @@ static int launch(const char* what, const Params& p, void* workspace, bool overl
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = overlap ? 1 : 0;
+  cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, few_kernel<T, D, MT>, maps, p);
   *join = ToJoin{maps.partial, maps.begun, split ? blocks : 0, maps.tpi};
   return check_launch(what);
 }
 
 template <typename T, int D>
-static int launch_rows(const char* what, const Params& p, int mt, void* workspace, bool overlap, ToJoin* join,
+static int launch_rows(const char* what, const Params& p, int mt, void* workspace, bool beside, ToJoin* join,
                        cudaStream_t stream) {
-  return mt == 1 ? launch<T, D, 1>(what, p, workspace, overlap, join, stream)
-                 : launch<T, D, 2>(what, p, workspace, overlap, join, stream);
+  return mt == 1 ? launch<T, D, 1>(what, p, workspace, beside, join, stream)
+                 : launch<T, D, 2>(what, p, workspace, beside, join, stream);
 }
 
 }  // namespace few
@@ -478,14 +479,14 @@ int64_t few_workspace(int head_dim) {
   return few::begun_bytes(n) + 2 * (int64_t)n * (int64_t)(head_dim == 64 ? sizeof(Slot<64, 32>) : sizeof(Slot<128, 32>));
 }
 
-int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, bool overlap, ToJoin* join,
+int launch_few(const char* what, const Params& p, int64_t rows, int dtype, void* workspace, bool beside, ToJoin* join,
                FewShape* shape, cudaStream_t s) {
   const int mt = shape->rows16 = rows <= 16 ? 1 : 2;
   if (dtype == JO_DTYPE_BF16)
-    return p.head_dim == 64 ? few::launch_rows<__nv_bfloat16, 64>(what, p, mt, workspace, overlap, join, s)
-                            : few::launch_rows<__nv_bfloat16, 128>(what, p, mt, workspace, overlap, join, s);
-  return p.head_dim == 64 ? few::launch_rows<__half, 64>(what, p, mt, workspace, overlap, join, s)
-                          : few::launch_rows<__half, 128>(what, p, mt, workspace, overlap, join, s);
+    return p.head_dim == 64 ? few::launch_rows<__nv_bfloat16, 64>(what, p, mt, workspace, beside, join, s)
+                            : few::launch_rows<__nv_bfloat16, 128>(what, p, mt, workspace, beside, join, s);
+  return p.head_dim == 64 ? few::launch_rows<__half, 64>(what, p, mt, workspace, beside, join, s)
+                          : few::launch_rows<__half, 128>(what, p, mt, workspace, beside, join, s);
 }
 
 int few_last_fault(int reset) {
