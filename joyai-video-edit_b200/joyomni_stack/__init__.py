@@ -10,4 +10,7 @@ def __getattr__(name):
     if name in ("StackConfig", "Stack", "Block", "LayerKV", "rope_tables"):
         from . import mmdit
         return getattr(mmdit, name)
+    if name in ("SessionCache", "SessionAttention"):
+        from . import sessions
+        return getattr(sessions, name)
     raise AttributeError(name)
