@@ -248,8 +248,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           t.kfirst = s.r.first;
           t.b = s.b;
           t.h = s.h;
-          t.edge = task_visible(p, t, 0) / kKeys;
-          t.end[0] = max(s.a, min(s.e, max(1, div_up(task_visible(p, t, min(t.ntok, N * tpt) - 1), kKeys))));
+          t.edge = (uint32_t)task_visible(p, t, 0) / kKeys;
+          t.end[0] = max(s.a, min(s.e, (int)max(1u, ((uint32_t)task_visible(p, t, min(t.ntok, N * tpt) - 1) + kKeys - 1) / kKeys)));
           t.end[1] = t.ntok > N * tpt ? s.e : s.a;
           t.slot = s.whole() ? -1 : 2 * unit + (s.a == 0 ? 1 : 0);
           if (s.a == 0 && s.e < s.steps)       // only the last piece ends inside an item

@@ -80,8 +80,8 @@ template <int KEYS, int LEAD, int MIN>
 struct Work {
   // Steps of item i: at least one, so that rows that see no key are written too.
   static __device__ __forceinline__ int steps(const Params& p, const Request& r, int i, int tpi) {
-    const int last = (int)min((long long)r.n, (i + 1LL) * tpi) - 1;
-    return max(1, div_up(visible(p, r, last), KEYS));
+    const int last = min(r.n, (i + 1) * tpi) - 1;      // (rows are below 2^30, an item's tokens below 2^10)
+    return max(1u, ((uint32_t)visible(p, r, last) + KEYS - 1) / KEYS);
   }
 
   // The even division of `total` units over `blocks` ranges.
@@ -128,9 +128,8 @@ struct Work {
 
   // Units of one key head of a request, by one thread or by a warp.
   static __device__ __forceinline__ long long head_units(const Params& p, const Request& r, int tpi, int from, int by) {
-    const int ni = div_up(r.n, tpi);
     long long u = 0;
-    for (int q = from; q < ni; q += by) u += LEAD + steps(p, r, q, tpi);
+    for (int q = from; q * tpi < r.n; q += by) u += LEAD + steps(p, r, q, tpi);
     return u;
   }
 
@@ -224,7 +223,7 @@ struct Work {
       long long off = f.off - h * f.per_head;                // units into the key head's items
       for (int q0 = 0;; q0 += 32) {
         const int q = q0 + lane;
-        const int n = (long long)q * tpi < r.n ? steps(p, r, q, tpi) : 0;
+        const int n = q * tpi < r.n ? steps(p, r, q, tpi) : 0;
         int inc = n ? LEAD + n : 0;      // (32 items of at most 2^24 + LEAD units)
         const int u = inc;
         if (r.n > tpi) {
@@ -251,7 +250,7 @@ struct Work {
           }
           break;
         }
-        if (q0 + 32LL >= r.n) break;     // (not reached: the cut lies in the request)
+        if (q0 + 32 >= r.n) break;       // (not reached: the cut lies in the request)
         off -= __shfl_sync(0xffffffffu, inc, 31);
       }
     }
@@ -292,20 +291,17 @@ struct Work {
   struct Walk {
     const Params& p;
     const Near& near;
-    int tpi, k, b, h, i, step, ni;
+    int tpi, k, b, h, i, step;
     long long at, end;
     Request r;
     // (The range's first request is the first of the near ones: it has rows.)
     __device__ Walk(const Params& p_, int tpi_, const Near& near_, const Range& g)
         : p(p_), near(near_), tpi(tpi_), k(0), b(g.b), h(g.h), i(g.i), step(g.step), at(g.begin), end(g.end) {
-      if (at < end) {
-        r = near.r[0];
-        ni = div_up(r.n, tpi);
-      }
+      if (at < end) r = near.r[0];
     }
     __device__ void advance() {
       step = 0;
-      if (++i < ni) return;
+      if (++i * tpi < r.n) return;
       i = 0;
       if (++h < p.kv_heads) return;
       h = 0;
@@ -321,7 +317,6 @@ struct Work {
         }
         if (r.n == 0) at = end;
       }
-      ni = div_up(r.n, tpi);
     }
     __device__ bool next(Piece& s) {
       while (at < end) {
