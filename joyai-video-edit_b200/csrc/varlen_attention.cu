@@ -48,9 +48,11 @@ constexpr int kThreads = 384;
 // (329 MB) 0.85 and 0.94.
 constexpr int kPairRows = 2048;
 constexpr int64_t kPairBytes = 192LL << 20;
-constexpr int kLead = 2;                 // steps that an item's beginning and end cost
-constexpr int kMin = 3;                  // steps of the shortest piece
-using Steps = Work<kKeys, kLead, kMin>;
+// Steps that an item's beginning and end cost; steps of the shortest piece; items
+// that are never cut.  (Beginnings at 1, 3, 4, pieces of 1, 3, 4: ragged prompts
+// 212-234 us against 209, mixed chunks 52-57 against 53.)
+constexpr int kLead = 2, kMin = 2, kWhole = 3;
+using Steps = Work<kKeys, kLead, kMin, kWhole>;
 using Range = Steps::Range;
 using Piece = Steps::Piece;
 using Walk = Steps::Walk;
@@ -551,9 +553,15 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         const bool edge = j >= first;
         const int lim = limit - j * kKeys;
         if (edge) {
+          // a warp's rows share most of the edge: 32 keys that all of them see are left alone
+          const int least = __reduce_min_sync(0xffffffffu, lim);
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= lim) x[i] = -INFINITY;
+          for (int q = 0; q < 128; q += 32)
+            if (least < q + 32) {
+#pragma unroll
+              for (int i = q; i < q + 32; ++i)
+                if (i >= lim) x[i] = -INFINITY;
+            }
         }
         float mq[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -731,8 +739,7 @@ static int64_t tile_workspace(int head_dim) {
   return begun_bytes(n) +
          2 * (int64_t)n * (int64_t)(head_dim == 64 ? sizeof(Slot<64, 2 * kRows>) : sizeof(Slot<128, 2 * kRows>));
 }
-// An item has a cut inside only if it is long enough to have one away from its edges.
-static bool tiles_split(int64_t max_keys) { return max_keys > (2 * kMin - 1) * kKeys; }
+static bool tiles_split(int64_t max_keys) { return max_keys > kWhole * kKeys; }
 static int64_t workspace_bytes_for(int64_t max_keys, int head_dim) {
   return tiles_split(max_keys) || few_splits(max_keys) ? tile_workspace(head_dim) + few_workspace(head_dim) : 0;
 }

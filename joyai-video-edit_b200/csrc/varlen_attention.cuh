@@ -74,9 +74,10 @@ __device__ __forceinline__ long long div_floor(long long a, long long b) {
 }
 
 // KEYS keys of a step.  Beginning and ending an item costs as much as LEAD steps,
-// which count as units of work too.  A cut closer than MIN steps to an item's
-// edge moves to the edge: a shorter piece would cost more to join than to compute.
-template <int KEYS, int LEAD, int MIN>
+// which count as units of work too.  A cut closer than MIN steps to an item's edge
+// moves to the edge: a shorter piece would cost more to join than to compute; and
+// so does any cut in an item of at most WHOLE steps.
+template <int KEYS, int LEAD, int MIN, int WHOLE>
 struct Work {
   // Steps of item i: at least one, so that rows that see no key are written too.
   static __device__ __forceinline__ int steps(const Params& p, const Request& r, int i, int tpi) {
@@ -237,10 +238,10 @@ struct Work {
         if (hit) {
           if (lane == __ffs(hit) - 1) {
             long long step = off - (inc - u) - LEAD;
-            if (step < MIN) {
+            if (step < MIN || (n <= WHOLE && 2 * step < n)) {
               f.at -= step + LEAD;
               step = 0;
-            } else if (n - step < MIN) {
+            } else if (n - step < MIN || n <= WHOLE) {
               f.at += n - step;
               step = n;
             }
