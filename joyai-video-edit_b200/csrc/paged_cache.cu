@@ -67,7 +67,8 @@ __device__ __forceinline__ longlong2 block_scan(longlong2 v, longlong2* warp_sum
 // starts at one of its new tokens, so the thread of that token writes the
 // table entry, and a token's own slot follows from the free list without
 // reading what another thread writes.  Latency-bound: a launch and a chain of
-// a few dependent loads, whatever the sizes.
+// a few dependent loads, whatever the sizes: 3.3 us for 48 requests of one token,
+// 3.9 us for 300 requests and 25093 places, launch included.
 __global__ void __launch_bounds__(kThreads) layout_kernel(const LayoutParams p) {
   __shared__ longlong2 warp_sums[kThreads / 32];
   __shared__ i64 s_start[kChunk];      // first token of the request
@@ -164,8 +165,8 @@ struct WriteParams {
 };
 
 // A thread takes the same 16-byte vector of K and of V of kTokens tokens, all loads before the first store: bound by HBM, and four
-// loads in flight per thread keep it busy (one token a thread: 21.3 us for 11042
-// tokens of 10 heads of 128, 5.3 TB/s).
+// loads in flight per thread keep it busy.  11042 tokens of 10 heads of 128: 20.0
+// us, 5.65 TB/s (one token a thread 21.3 us, four 20.4).
 constexpr int kTokens = 2;
 __global__ void __launch_bounds__(kThreads) write_kernel(const WriteParams p) {
   const uint32_t x = blockIdx.y * blockDim.x + threadIdx.x;
