@@ -8,12 +8,12 @@
 // and four warps on mma.sync (m16n8k16: its 16 rows fit a group, where the 128 of
 // a tcgen05 tile would be mostly empty).  Of a step's scores each warp has 16
 // keys, of its output a quarter of the columns; the weights change hands in
-// shared memory, with one barrier a step.  The steps of all items are shared out
+// shared memory, with two barriers a step.  The steps of all items are shared out
 // evenly over the blocks (varlen_attention.cuh).
 //
 // Measured, the join included: one token over 131071 cached ones (32 heads over 8
-// of 128, 537 MB) 97 us, 5.5 TB/s; 64 single tokens over 54480 (224 MB) 48.5 us;
-// one over 300 (14 heads over 2 of 64) 7.6 us, nearly all of it latency.
+// of 128, 537 MB) 98.5 us, 5.45 TB/s; 64 single tokens over 54480 (224 MB) 48.8 us;
+// one over 300 (14 heads over 2 of 64) 8.0 us, nearly all of it latency.
 #include "varlen_attention.cuh"
 
 namespace jo {
@@ -25,8 +25,7 @@ constexpr int kWarps = 4;                // warps that compute
 constexpr int kThreads = 32 * (kWarps + 1);
 // Steps that an item's beginning and end cost; steps of the shortest piece; items
 // that are never cut (a join takes as long as some seven steps: 300 tokens in one
-// piece 7.6 us, in three 10.1; 4000 tokens 11.3 us against 12.4 in pieces of four
-// at least).
+// piece 7.6 us, in three 10.1; 4000 tokens 11.3 us, in pieces of four at least 12.4).
 constexpr int kLead = 2, kMin = 2, kWhole = 7;
 constexpr int kBlocksPerSm = 2;
 
@@ -43,7 +42,7 @@ template <int D, int MT> struct Cfg {
   static constexpr int TILE = HALVES * HALF;                 // K or V of a step
   static constexpr int ST = D == 128 ? 3 : 6;                // steps in flight: 96 KB
   static constexpr int Q0 = ST * 2 * TILE;                   // Q: R rows, 16-byte pieces turned as the swizzle does
-  static constexpr int P0 = Q0 + R * D * 2;                  // weights: two buffers of R rows of 64 keys, likewise
+  static constexpr int P0 = Q0 + R * D * 2;                  // weights: R rows of 64 keys, likewise; rounded, then the rest
   static constexpr int P_BYTES = R * kKeys * 2;
   static constexpr int BARS = P0 + 2 * P_BYTES;
   static constexpr int NEAR = BARS + 128;
@@ -215,7 +214,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
         ok = ok && __all_sync(0xffffffffu, mbar_wait(FULL(st), (it / ST) & 1, abort_flag, &g_fault, 102));
         const uint32_t ks = ring + st * 2 * C::TILE, vs = ks + C::TILE;
         const int key0 = j * kKeys + warp * 16;              // this warp's keys
-        const uint32_t pbuf = ps + (it & 1) * C::P_BYTES;
         float x[MT][2][4], x2[MT][2][4];                     // even and odd products apart: half the chain
 #pragma unroll
         for (int t = 0; t < MT; ++t)
@@ -276,8 +274,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
           fence_async_smem();                                // the next copy into this place comes after these writes
           bad = __any_sync(0xffffffffu, bad);
         }
-        // The maximum only moves when it grows by more than 2^8 somewhere: the
-        // weights are made with the old one, and again in the rare other case.
+        // The maximum only moves when it grows by more than 2^8 somewhere.
         float top[MT][2];
         bool raise = false;
 #pragma unroll
@@ -289,28 +286,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
             top[t][e] = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * c;
             raise |= top[t][e] > m[t][e] + 8.f;
           }
-        float sum[MT][2];
-        auto weigh = [&]() {
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = t * 16 + e * 8 + qr;
-              sum[t][e] = 0.f;
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const float a = ex2(fmaf(x[t][n][2 * e], c, -m[t][e])), b = ex2(fmaf(x[t][n][2 * e + 1], c, -m[t][e]));
-                sum[t][e] += a + b;
-                // rounded to the tensors' type for the product with V; the sum is of the unrounded ones
-                *reinterpret_cast<uint32_t*>(smem + (pbuf - ring) + r * 128 + (((warp * 2 + n) ^ (r & 7)) << 4) + qc * 2) =
-                    pack2<T>(a, b);
-              }
-            }
-        };
-        weigh();
-        if (team_any(raise)) {
-          // all are past the step before, so its buffer has room for the maxima
-          float* tops = reinterpret_cast<float*>(smem + C::P0 + ((it + 1) & 1) * C::P_BYTES);
+        if (team_any(raise)) {                               // (all are past the step before: its weights' place is free)
+          float* tops = reinterpret_cast<float*>(smem + C::P0);
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -333,9 +310,31 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
                 o[t][n][2 * e + 1] *= alpha;
               }
             }
-          weigh();
           team_sync();
         }
+        // The weights, as the sum of two numbers of the tensors' type, so that the
+        // product with V keeps 16 bits of them and more.  (Rounded once, they made the
+        // result's error 1.4 times that of rounding it; this costs 0.4 us of 8 at one
+        // short request and 0.5-1 % at the others.)
+        float sum[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = t * 16 + e * 8 + qr;
+            sum[t][e] = 0.f;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const float a = ex2(fmaf(x[t][n][2 * e], c, -m[t][e])), b = ex2(fmaf(x[t][n][2 * e + 1], c, -m[t][e]));
+              sum[t][e] += a + b;
+              const uint32_t hi = pack2<T>(a, b);
+              const float2 h = unpack2<T>(hi);
+              unsigned char* at = smem + C::P0 + r * 128 + (((warp * 2 + n) ^ (r & 7)) << 4) + qc * 2;
+              *reinterpret_cast<uint32_t*>(at) = hi;
+              *reinterpret_cast<uint32_t*>(at + C::P_BYTES) = pack2<T>(a - h.x, b - h.y);
+            }
+          }
+        team_sync();
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           l[t][0] += sum[t][0];
@@ -344,10 +343,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
         if (!bad) {
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k) {
-            uint32_t a[MT][4];
+            uint32_t a[MT][4], rest[MT][4];
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-              ldsm4(pbuf + (t * 16 + arow) * 128 + (((k * 2 + acol) ^ (arow & 7)) << 4), a[t]);
+            for (int t = 0; t < MT; ++t) {
+              const uint32_t at = ps + (t * 16 + arow) * 128 + (((k * 2 + acol) ^ (arow & 7)) << 4);
+              ldsm4(at, a[t]);
+              ldsm4(at + C::P_BYTES, rest[t]);
+            }
 #pragma unroll
             for (int n = 0; n < NW / 2; ++n) {
               const int col = warp * NW + 2 * n + vcol;      // 8-column block
@@ -357,6 +359,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
               for (int t = 0; t < MT; ++t) {
                 mma16816<T>(o[t][2 * n], a[t], b[0], b[1]);
                 mma16816<T>(o[t][2 * n + 1], a[t], b[2], b[3]);
+                mma16816<T>(o[t][2 * n], rest[t], b[0], b[1]);
+                mma16816<T>(o[t][2 * n + 1], rest[t], b[2], b[3]);
               }
             }
           }
@@ -375,8 +379,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
                 for (int e = 0; e < 2; ++e)
                   if (j * kKeys + k < limit[t][e]) {
                     const int r = t * 16 + e * 8 + qr;
-                    const float w = to_f32(*reinterpret_cast<const T*>(smem + (pbuf - ring) + r * 128 +
-                                                                       (((k >> 3) ^ (r & 7)) << 4) + (k & 7) * 2));
+                    const T* at = reinterpret_cast<const T*>(smem + C::P0 + r * 128 + (((k >> 3) ^ (r & 7)) << 4) + (k & 7) * 2);
+                    const float w = to_f32(at[0]) + to_f32(at[C::P_BYTES / 2]);
                     o[t][n][2 * e] = fmaf(w, f.x, o[t][n][2 * e]);
                     o[t][n][2 * e + 1] = fmaf(w, f.y, o[t][n][2 * e + 1]);
                   }
