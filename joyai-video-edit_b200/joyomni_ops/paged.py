@@ -33,6 +33,8 @@ _S4 = struct.Struct("4q").pack        # strides for the C ABI's const int64_t*
 _S6 = struct.Struct("6q").pack
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch._C._cuda_getDevice
+_layout, _write, _paged, _prompt = (_L.jo_paged_layout, _L.jo_paged_kv_write, _L.jo_paged_attention,
+                                    _L.jo_prompt_attention)
 
 # These calls take a few microseconds on the GPU, so what the host does for one
 # counts: arguments are looked at in one expression each, and only a refusal
@@ -44,15 +46,10 @@ def _chk(cond: bool, msg: str) -> None:
         raise RuntimeError(msg)
 
 
-def _call(f, idx: int, *args) -> None:
-    """f(*args, stream) on the current stream of device `idx`, which is current meanwhile."""
-    if _device() == idx:
-        status = f(*args, _stream(idx))
-    else:
-        with torch.cuda.device(idx):
-            status = f(*args, _stream(idx))
-    if status:
-        _check(status)
+def _on(idx: int, f, *args, **kw):
+    """f(*args, **kw) with device `idx` current."""
+    with torch.cuda.device(idx):
+        return f(*args, **kw)
 
 
 def _ints(t: torch.Tensor, name: str, dim: int, dtype: torch.dtype, idx: int) -> None:
@@ -118,9 +115,13 @@ def paged_layout(cached_lens, new_lens, block_tables, free_blocks, page_size: in
             and slots.is_contiguous() and pos.is_contiguous()):
         raise RuntimeError(f"out must hold contiguous tensors on cuda:{idx} of PagedLayout.empty({B}, {num_tokens}, ...)'s "
                            "sizes and types")
-    _call(_L.jo_paged_layout, idx, cached_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(),
-          free_blocks.data_ptr(), B, width, block_tables.stride(0) if B > 1 else width, free_blocks.numel(), page_size,
-          num_tokens, starts.data_ptr(), lens.data_ptr(), slots.data_ptr(), pos.data_ptr(), needed.data_ptr())
+    if _device() != idx:
+        return _on(idx, paged_layout, cached_lens, new_lens, block_tables, free_blocks, page_size, num_tokens, out=out)
+    status = _layout(cached_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(), B, width,
+                     block_tables.stride(0) if B > 1 else width, free_blocks.numel(), page_size, num_tokens,
+                     starts.data_ptr(), lens.data_ptr(), slots.data_ptr(), pos.data_ptr(), needed.data_ptr(), _stream(idx))
+    if status:
+        _check(status)
     return out
 
 
@@ -153,9 +154,12 @@ def paged_kv_write(key, value, key_cache, value_cache, slots) -> None:
             and slots.dtype is _I64 and slots.get_device() == idx and slots.is_contiguous() and slots.shape == shape[:1]):
         _refuse_write(key, value, key_cache, value_cache, slots)
     T, H, D = shape
-    _call(_L.jo_paged_kv_write, idx, key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-          slots.data_ptr(), T, H, D, cs[0], cs[1], _S4(a[0], a[1], b[0], b[1]),
-          _S6(c[0], c[1], c[2], d[0], d[1], d[2]), code)
+    if _device() != idx:
+        return _on(idx, paged_kv_write, key, value, key_cache, value_cache, slots)
+    status = _write(key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), slots.data_ptr(), T, H, D,
+                    cs[0], cs[1], _S4(a[0], a[1], b[0], b[1]), _S6(c[0], c[1], c[2], d[0], d[1], d[2]), code, _stream(idx))
+    if status:
+        _check(status)
 
 
 def _refuse_write(key, value, key_cache, value_cache, slots) -> None:
@@ -252,11 +256,17 @@ def paged_attention(query, key_cache, value_cache, block_tables, query_starts, k
     o = _out(query, out)
     ws, ws_bytes, _keep = _workspace(workspace, idx, width * cs[1], D)
     e = o.stride()
-    _call(_L.jo_paged_attention, idx, query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-          block_tables.data_ptr(), query_starts.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), T, B, H, cs[2], D, cs[0],
-          cs[1], width, block_tables.stride(0) if B > 1 else width, _S4(a[0], a[1], e[0], e[1]),
-          _S6(c[0], c[1], c[2], d[0], d[1], d[2]), bool(causal), 1.0 / math.sqrt(D) if scale is None else scale,
-          T if max_query_len is None else max_query_len, code, ws, ws_bytes)
+    if _device() != idx:
+        return _on(idx, paged_attention, query, key_cache, value_cache, block_tables, query_starts, kv_lens, causal=causal,
+                   scale=scale, max_query_len=max_query_len, out=o, workspace=_keep)
+    status = _paged(query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+                    query_starts.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), T, B, H, cs[2], D, cs[0], cs[1], width,
+                    block_tables.stride(0) if B > 1 else width, _S4(a[0], a[1], e[0], e[1]),
+                    _S6(c[0], c[1], c[2], d[0], d[1], d[2]), 1 if causal else 0,
+                    1.0 / math.sqrt(D) if scale is None else scale, T if max_query_len is None else max_query_len, code, ws,
+                    ws_bytes, _stream(idx))
+    if status:
+        _check(status)
     return o
 
 
@@ -299,9 +309,13 @@ def prompt_attention(query, key, value, seq_starts, *, causal: bool = True, scal
     o = _out(query, out)
     ws, ws_bytes, _keep = _workspace(workspace, idx, T, D)
     e = o.stride()
-    _call(_L.jo_prompt_attention, idx, query.data_ptr(), key.data_ptr(), value.data_ptr(), seq_starts.data_ptr(),
-          o.data_ptr(), T, seq_starts.numel() - 1, H, ks[1], D, _S4(a[0], a[1], e[0], e[1]),
-          _S4(b[0], b[1], c[0], c[1]), bool(causal), 1.0 / math.sqrt(D) if scale is None else scale, code, ws, ws_bytes)
+    if _device() != idx:
+        return _on(idx, prompt_attention, query, key, value, seq_starts, causal=causal, scale=scale, out=o, workspace=_keep)
+    status = _prompt(query.data_ptr(), key.data_ptr(), value.data_ptr(), seq_starts.data_ptr(), o.data_ptr(), T,
+                     seq_starts.numel() - 1, H, ks[1], D, _S4(a[0], a[1], e[0], e[1]), _S4(b[0], b[1], c[0], c[1]),
+                     1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale, code, ws, ws_bytes, _stream(idx))
+    if status:
+        _check(status)
     return o
 
 
