@@ -618,3 +618,18 @@ def test_chunks_and_single_tokens_together(jo, cuda, H, Hk, D):
     for _ in range(3):
         c.check(c.run(jo))
     jo.check_gemm_fault()
+
+
+@pytest.mark.parametrize("H,Hk,new,cached", [
+    (16, 4, [65, 129, 67, 64, 8, 200], [3000, 0, 500, 77, 64, 1]), (16, 4, [131], [2000]), (8, 8, [257, 513, 300], [0, 9, 400]),
+    (7, 1, [37, 40, 36, 73], [100, 0, 1000, 5]), (10, 2, [53, 50, 51], [0, 700, 64]),
+])
+def test_last_rows_of_chunks(jo, cuda, H, Hk, new, cached):
+    """Chunks a few rows longer than whole tiles of rows."""
+    for D, dt in ((128, "bf16"), (64, "f16")):
+        for causal in (True, False):
+            c = Case(cuda, cached, new, H, Hk, D, 16, dt, seed=24)
+            c.check(c.run(jo, causal), causal)
+    kv = [max(0, n - 30) for n in new]                       # the first rows see nothing
+    c = Case(cuda, None, new, H, Hk, 128, 32, seed=25, kv=kv)
+    c.check(c.run(jo))
