@@ -720,17 +720,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p, c
   __shared__ float shared[kJoinWarps][10][32];
   wait_for_primary();
   launch_dependents();
-  const int c = blockIdx.x, y = blockIdx.y;
-  if (c < tiles.blocks) {
-    if (y < join_y(D, TR, 1)) join_item<T, D, TR, kRows, 1>(p, tiles, c, y, shared);
-  } else if (y < join_y(D, 32, 2)) {
-    join_item<T, D, 32, FR, 2>(p, few, c - tiles.blocks, y, shared);
-  }
+  constexpr int TY = join_y(D, TR, 1), FY = join_y(D, 32, 2);
+  const int i = blockIdx.x, tile_blocks = tiles.blocks * TY;
+  if (i < tile_blocks) join_item<T, D, TR, kRows, 1>(p, tiles, i / TY, i % TY, shared);
+  else join_item<T, D, 32, FR, 2>(p, few, (i - tile_blocks) / FY, (i - tile_blocks) % FY, shared);
 }
 template <typename T, int D, int TR, int FR>
 static void launch_join(const Params& p, const ToJoin& tiles, const ToJoin& few, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles.blocks + few.blocks), tiles.blocks ? join_y(D, TR, 1) : join_y(D, 32, 2));
+  cfg.gridDim = dim3((unsigned)(tiles.blocks * join_y(D, TR, 1) + few.blocks * join_y(D, 32, 2)));
   cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];

@@ -387,8 +387,9 @@ struct ToJoin {
 // and 8 columns of it (y and the team's place in the block enumerate them), each
 // lane one row; the team's warps share out the partial results and warp 0 adds
 // theirs up.  Latency-bound: the reads of four partial results are in flight at a
-// time (six, and more or larger blocks, measured slower: 54 against 49 us for 64
-// single tokens over 54480 cached ones, most of whose blocks find nothing to do).
+// time.  Most blocks find nothing to do, and more or larger ones measured slower (54
+// against 49 us for 64 single tokens over 54480 cached ones), fewer that look for
+// work too (50.4).
 constexpr int kJoinWarps = 8;
 template <typename T, int D, int R, int TILE, int TEAM>
 __device__ __forceinline__ void join_item(const Params& p, const ToJoin& j, int c, int y, float (*shared)[10][32]) {
@@ -399,7 +400,6 @@ __device__ __forceinline__ void join_item(const Params& p, const ToJoin& j, int 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp % TEAM;
   const int w = y * (kJoinWarps / TEAM) + warp / TEAM;
   const int col = (w % (D / 8)) * 8, r = (w / (D / 8)) * 32 + lane;
-  if (w >= R / 32 * (D / 8)) return;     // (the whole block: R / 32 * D / 8 is a multiple of its teams)
   int tok, head;
   const bool valid = row_place<TILE>(r, p.group, j.tpt, me.n, tok, head);
   float m = kNoMax, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
