@@ -927,7 +927,8 @@ int jo_paged_attention(const void* q, const void* key_cache, const void* value_c
   JO_REQUIRE(num_blocks >= 0 && num_blocks < (1LL << 31) && table_width >= 0 && table_width < (1LL << 31) &&
                  table_stride >= 0 && table_width * page_size <= (1LL << 30),
              JO_ERR_INVALID, "%s: invalid cache or block table shape", what);
-  vattn::Params p{q, key_cache, value_cache, out, query_starts, kv_lens, block_tables,
+  // (a table without columns is never read, but says that there is one)
+  vattn::Params p{q, key_cache, value_cache, out, query_starts, kv_lens, table_width > 0 ? block_tables : query_starts,
                   r[0], r[1], c[0], c[1], c[2], c[3], c[4], c[5], r[2], r[3], table_stride};
   p.num_blocks = (int)num_blocks;
   p.page = (int)page_size;
@@ -935,7 +936,8 @@ int jo_paged_attention(const void* q, const void* key_cache, const void* value_c
   p.causal = causal != 0;
   int st = vattn::check(what, p, tokens, batch, heads, kv_heads, head_dim, scale, dtype);
   if (st != JO_OK) return st;
-  JO_REQUIRE(tokens == 0 || batch == 0 || (kv_lens && block_tables && (num_blocks == 0 || (key_cache && value_cache))),
+  JO_REQUIRE(tokens == 0 || batch == 0 || (kv_lens && (block_tables || table_width == 0) &&
+                                            (num_blocks == 0 || (key_cache && value_cache))),
              JO_ERR_INVALID, "%s: null tensor pointer", what);
   return vattn::launch(what, p, max_query_len, dtype, workspace, workspace_bytes, stream);
 }

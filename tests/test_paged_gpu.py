@@ -297,6 +297,19 @@ def test_empty_requests_and_rows_of_none(jo, cuda):
     assert none.shape == (0, 4, 64)
 
 
+def test_empty_tables_and_caches(jo, cuda):
+    """A table without columns, a cache without blocks: every row is zero."""
+    for n in (1, 100):
+        q = torch.randn(n, 4, 64, device=cuda).to(torch.bfloat16)
+        starts, lens = i32([0, n], cuda), i32([n], cuda)
+        cache = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16, device=cuda)
+        none = torch.zeros(1, 0, dtype=torch.int32, device=cuda)
+        assert bool((jo.paged_attention(q, cache, cache, none, starts, lens) == 0).all())
+        table = torch.zeros(1, 8, dtype=torch.int32, device=cuda)
+        assert bool((jo.paged_attention(q, cache[:0], cache[:0], table, starts, lens) == 0).all())
+        jo.paged_kv_write(q[:, :2], q[:, 2:], cache[:0], cache[:0], torch.arange(n, device=cuda))
+
+
 @pytest.mark.parametrize("hint", [None, 1, 4, 1000])
 def test_max_query_len_only_hints(jo, cuda, hint):
     c = Case(cuda, [900, 50, 3, 0], [3, 1, 200, 17], 8, 2, 128, 64, seed=9)
@@ -632,4 +645,16 @@ def test_last_rows_of_chunks(jo, cuda, H, Hk, new, cached):
             c.check(c.run(jo, causal), causal)
     kv = [max(0, n - 30) for n in new]                       # the first rows see nothing
     c = Case(cuda, None, new, H, Hk, 128, 32, seed=25, kv=kv)
+    c.check(c.run(jo))
+
+
+@pytest.mark.parametrize("B,most", [(161, 1), (600, 1), (1300, 3), (500, 60)])
+def test_many_requests(jo, cuda, B, most):
+    """More requests than a block has threads, idle ones among them."""
+    r = random.Random(B)
+    new = [r.randrange(0, most + 1) if i % 3 else 0 for i in range(B)]
+    c = Case(cuda, [r.choice([0, 1, 20, r.randrange(400)]) for _ in range(B)], new, 4, 2, 64, 16, seed=26)
+    got = c.run(jo, max_query_len=most)
+    c.check(got)
+    assert torch.equal(got, c.run(jo, max_query_len=most))
     c.check(c.run(jo))
