@@ -402,6 +402,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
           if ((lane & 3) == 0) sums[warp * R + t * 16 + e * 8 + qr] = l[t][e];
         }
       team_sync();
+      float seen = 0.f;                                      // NaN where a sum is not finite
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NW; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) seen = fmaf(o[t][n][i], 0.f, seen);
+      const bool odd = __any_sync(0xffffffffu, seen != seen);
       const bool whole = s.whole();
       Slot<D, 32>& slot = static_cast<Slot<D, 32>*>(maps.partial)[2 * blockIdx.x + (s.a == 0 ? 1 : 0)];
 #pragma unroll
@@ -412,6 +420,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
           float sum = 0.f;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) sum += sums[w * R + r];
+          if (odd) {
+            const Values values(p, s.r.first, s.b, s.h);
+#pragma unroll
+            for (int n = 0; n < NW; ++n) {
+              float x[8];
+              odd_values<T>(values, (warp * NW + n) * 8, s.a * kKeys, some, min(s.e * kKeys, most), limit[t][e], x);
+              o[t][n][2 * e] = with_odd(o[t][n][2 * e], x[qc], sum);
+              o[t][n][2 * e + 1] = with_odd(o[t][n][2 * e + 1], x[qc + 1], sum);
+            }
+          }
           if (tok >= ntok) continue;
           if (whole) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
