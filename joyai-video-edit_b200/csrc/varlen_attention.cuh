@@ -390,7 +390,9 @@ struct ToJoin {
 // time.  Most blocks find nothing to do, and more or larger ones measured slower (54
 // against 49 us for 64 single tokens over 54480 cached ones), fewer that look for
 // work too (50.4).
+// (Factors stop at kLeast, so that an infinity stays one however small its part.)
 constexpr int kJoinWarps = 8;
+constexpr float kLeast = 1.17549435e-38f;   // the smallest normal number
 template <typename T, int D, int R, int TILE, int TEAM>
 __device__ __forceinline__ void join_item(const Params& p, const ToJoin& j, int c, int y, float (*shared)[10][32]) {
   static_assert(kJoinWarps % TEAM == 0, "");
@@ -420,7 +422,7 @@ __device__ __forceinline__ void join_item(const Params& p, const ToJoin& j, int 
 #pragma unroll
     for (int k = 0; k < DEEP; ++k) {
       if (i0 + k >= hi || ml[k].y == 0.f) continue;      // a row without a visible key there has no O either
-      const float mn = fmaxf(m, ml[k].x), a = ex2(m - mn), b = ex2(ml[k].x - mn);
+      const float mn = fmaxf(m, ml[k].x), a = fmaxf(ex2(m - mn), kLeast), b = fmaxf(ex2(ml[k].x - mn), kLeast);
       m = mn;
       l = l * a + ml[k].y * b;
       const float v[8] = {x[k].x, x[k].y, x[k].z, x[k].w, y[k].x, y[k].y, y[k].z, y[k].w};
@@ -439,7 +441,7 @@ __device__ __forceinline__ void join_item(const Params& p, const ToJoin& j, int 
     for (int k = 1; k < TEAM; ++k) {
       float(*other)[32] = shared[warp + k];
       if (other[1][lane] == 0.f) continue;
-      const float mo = other[0][lane], mn = fmaxf(m, mo), a = ex2(m - mn), b = ex2(mo - mn);
+      const float mo = other[0][lane], mn = fmaxf(m, mo), a = fmaxf(ex2(m - mn), kLeast), b = fmaxf(ex2(mo - mn), kLeast);
       m = mn;
       l = l * a + other[1][lane] * b;
 #pragma unroll
@@ -504,7 +506,7 @@ __device__ __forceinline__ void kv_place(const Params& p, int first, int keys, i
 
 // ---------------------------------------------------- infinite values of V ----
 // An infinity in V that a row sees makes its result infinite, but in the products
-// a weight (or the rest of one) that is zero turns it into NaN.  V is not searched
+// a weight (or the rest of one) that rounds to zero turns it into NaN.  V is not searched
 // for them on the way: a piece whose sums hold a NaN, though its weights are
 // numbers, looks through the keys again when it ends and takes from there what its
 // columns see.  So only calls that meet infinities or NaN pay for it (the look at

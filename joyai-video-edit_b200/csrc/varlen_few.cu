@@ -402,14 +402,21 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
           if ((lane & 3) == 0) sums[warp * R + t * 16 + e * 8 + qr] = l[t][e];
         }
       team_sync();
-      float seen = 0.f;                                      // NaN where a sum is not finite
+      float total[MT][2];                                    // the rows' sums of weights
+      bool nan = false;                                      // in a row whose weights are numbers
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int n = 0; n < NW; ++n)
+        for (int e = 0; e < 2; ++e) {
+          float seen = 0.f;                                  // NaN where a sum is not finite
+          total[t][e] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) seen = fmaf(o[t][n][i], 0.f, seen);
-      const bool odd = __any_sync(0xffffffffu, seen != seen);
+          for (int w = 0; w < kWarps; ++w) total[t][e] += sums[w * R + t * 16 + e * 8 + qr];
+#pragma unroll
+          for (int n = 0; n < NW; ++n) seen = fmaf(o[t][n][2 * e], 0.f, fmaf(o[t][n][2 * e + 1], 0.f, seen));
+          nan |= seen != seen && total[t][e] > 0.f;
+        }
+      const bool odd = __any_sync(0xffffffffu, nan);
       const bool whole = s.whole();
       Slot<D, 32>& slot = static_cast<Slot<D, 32>*>(maps.partial)[2 * blockIdx.x + (s.a == 0 ? 1 : 0)];
 #pragma unroll
@@ -417,9 +424,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = t * 16 + e * 8 + qr, tok = r / p.group, g = r - tok * p.group;
-          float sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) sum += sums[w * R + r];
+          const float sum = total[t][e];
           if (odd) {
             const Values values(p, s.r.first, s.b, s.h);
 #pragma unroll

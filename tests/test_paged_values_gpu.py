@@ -66,6 +66,55 @@ def test_infinity_that_every_row_sees(jo, cuda, cached, new, H, Hk, D, dt):
                 check_columns(c, got, b, 0, n, want, causal)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("cached,new,H,Hk", [
+    ([200], [1], 8, 2), ([200, 300, 200], [1, 4, 2], 8, 2), ([5000], [1], 8, 2), ([200], [40], 4, 2), ([5000, 300], [100, 2], 8, 4),
+])
+def test_infinity_of_small_weight(jo, cuda, cached, new, H, Hk, dt):
+    """Keys whose scores lie 30, 60 and 200 below the others': their weights round to zero in 16 bits, the last
+    one in 32 too, and an infinite value still belongs to the sum."""
+    D = 128
+    for causal in (True, False):
+        c = Case(cuda, cached, new, H, Hk, D, 16, dt, seed=32, scale=0.125)
+        c.q[..., 0] = 8.0                                    # adds 8 * 0.125 * k[0] to every score
+        for b in range(len(new)):
+            c.ks[b][:, :, 0] = 0.0
+            at = torch.arange(c.kv[b], device=cuda)
+            c.kc[c.table[b].long()[at // 16], at % 16, :, 0] = 0.0
+            last = cached[b] - 1
+            for j, col, x, low in ((70, 3, INF, 30), (71, 17, -INF, 60), (last, 50, INF, 30), (72, 60, INF, 200),
+                                   (73, 61, INF, 30), (last - 1, 61, -INF, 30)):
+                put_k(c, b, j, 0, -float(low))
+                put_v(c, b, j, col, x)
+        want = {3: INF, 17: -INF, 50: INF, 60: INF, 61: NAN}
+        for got in (c.run(jo, causal), c.run(jo, causal, max_query_len=max(new))):
+            for b, n in enumerate(new):
+                check_columns(c, got, b, 0, n, want, causal)
+
+
+@pytest.mark.parametrize("big", [False, True])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_infinities_in_long_chunks(jo, cuda, dt, big):
+    """The same through the kernel in block pairs too: infinities that all rows see, and ones that only later rows do."""
+    c = Case(cuda, [300], [900], 12, 4, 128, 16, dt, seed=33, scale=0.125, **(large(4, 16) if big else {}))
+    c.q[..., 0] = 8.0
+    for j in range(0, c.kv[0], 16):
+        c.kc[c.table[0, j // 16].item(), :, :, 0] = 0.0
+    c.ks[0][:, :, 0] = 0.0
+    for j, col, x, low in ((40, 3, INF, 0), (290, 17, -INF, 0), (90, 50, INF, 30), (299, 100, -INF, 30), (300 + 500, 101, INF, 30),
+                           (300 + 601, 127, -INF, 0)):
+        put_k(c, 0, j, 0, -float(low))
+        put_v(c, 0, j, col, x)
+    for causal in (True, False):
+        got = c.run(jo, causal, max_query_len=900)
+        jo.check_gemm_fault()
+        want = {3: INF, 17: -INF, 50: INF, 100: -INF}
+        later = {101: INF, 127: -INF}
+        cuts = ((0, 500, {}), (500, 601, {101: INF}), (601, 900, later)) if causal else ((0, 900, later),)
+        for lo, hi, more in cuts:
+            check_columns(c, got, 0, lo, hi, {**want, **more}, causal)
+
+
 def test_nan_weights_stay_nan(jo, cuda):
     """A NaN score makes its row NaN, whatever V holds."""
     for new in ([1], [3], [70]):
