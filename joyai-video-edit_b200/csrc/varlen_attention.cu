@@ -29,8 +29,10 @@
 // reads besides its own 128 rows, what bounds it in the single form, is halved, and
 // twice as many steps are in flight.  The even block issues the MMAs.
 //   warps 0-7    softmax: one thread per row, P over S in tensor memory
-// The running maximum only moves when it grows by more than 2^8, so most steps
-// leave O alone.
+// The weights' reference only moves when the maximum has grown enough, so most steps
+// leave O alone.  They are rounded once to the tensors' type, as the matrix
+// instruction takes them: a second product for the rest, as in varlen_few.cu, would
+// double PV.  Results have 1.1-1.4 times the error of rounding them alone.
 //
 // What bounds it: for long requests the chain of a tile, softmax (1750 cycles), P
 // seen by the MMA warp (450), PV and the next QK into the place that P leaves
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       const int a = task.a, e = task.e, end = task.end[t], first = task.edge;
       const int k_tok = ti * tpt + row_tok;        // the row's token in the item
       const int limit = task_visible(p, task, min(k_tok, task.ntok - 1));
-      float m = kNoMax;                            // running max of s * c (may lag the true one by less than 8)
+      float m = kNoMax;                            // reference of the weights: lags behind the maximum of s * c
       float l = 0.f;                               // running sum
       bool ok = true;
       for (int j = a; j < e; ++j, ++it) {
@@ -599,9 +601,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         mq[0] = max3f(mq[0], x[124], x[125]);
         mq[1] = max3f(mq[1], x[126], x[127]);
         const float mt = max3f(mq[0], mq[1], fmaxf(mq[2], mq[3])) * c;
-        const bool need = mt > m + 8.f;
+        const bool need = mt > m + (Weight<T>::kUp + Weight<T>::kLag);
         const bool any_need = __any_sync(0xffffffffu, need);
-        const float m_new = need ? mt : m;
+        const float m_new = need ? mt - Weight<T>::kUp : m;
         const float alpha = ex2(m - m_new);        // 1 where the max is kept; 0 at the first visible key
         m = m_new;
         const float2 c2 = make_float2(c, c), mn2 = make_float2(-m, -m);

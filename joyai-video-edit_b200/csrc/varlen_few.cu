@@ -274,7 +274,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
           fence_async_smem();                                // the next copy into this place comes after these writes
           bad = __any_sync(0xffffffffu, bad);
         }
-        // The maximum only moves when it grows by more than 2^8 somewhere.
+        // m only moves when the maximum has grown by more than kLag somewhere.
+        constexpr float kGrown = Weight<T>::kUp + Weight<T>::kLag;
         float top[MT][2];
         bool raise = false;
 #pragma unroll
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
             float mx = fmaxf(fmaxf(x[t][0][2 * e], x[t][0][2 * e + 1]), fmaxf(x[t][1][2 * e], x[t][1][2 * e + 1]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             top[t][e] = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * c;
-            raise |= top[t][e] > m[t][e] + 8.f;
+            raise |= top[t][e] > m[t][e] + kGrown;
           }
         if (team_any(raise)) {                               // (all are past the step before: its weights' place is free)
           float* tops = reinterpret_cast<float*>(smem + C::P0);
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
               float mx = kNoMax;
 #pragma unroll
               for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, tops[w * R + t * 16 + e * 8 + qr]);
-              const float mn = mx > m[t][e] + 8.f ? mx : m[t][e], alpha = ex2(m[t][e] - mn);
+              const float mn = mx > m[t][e] + kGrown ? mx - Weight<T>::kUp : m[t][e], alpha = ex2(m[t][e] - mn);
               m[t][e] = mn;
               l[t][e] *= alpha;
 #pragma unroll
@@ -313,7 +314,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
           team_sync();
         }
         // The weights, as the sum of two numbers of the tensors' type, so that the
-        // product with V keeps 16 bits of them and more.  (Rounded once, they made the
+        // product with V keeps 16 bits of them and more (fp16: of those above 2^-20 of
+        // the largest; of smaller ones all multiples of 2^-35).  (Rounded once, they made the
         // result's error 1.4 times that of rounding it; this costs 0.4 us of 8 at one
         // short request and 0.5-1 % at the others.)
         float sum[MT][2];

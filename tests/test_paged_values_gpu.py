@@ -124,3 +124,57 @@ def test_nan_weights_stay_nan(jo, cuda):
         got = c.run(jo)
         assert bool(torch.isnan(got[0, 1]).all())
         assert bool((got[0, 0, 3] == INF).all()) and bool(torch.isfinite(got[0, 0, 4:]).all())
+
+
+# fp16 holds weights below 2^-14 with a fixed spacing.
+@pytest.mark.parametrize("below", [12.0, 14.0, 16.0, 17.375])
+@pytest.mark.parametrize("cached,new,H,Hk", [([1023], [1], 8, 2), ([700, 1023], [1, 2], 8, 2), ([20000], [1], 8, 2),
+                                             ([1023], [100], 4, 4), ([511, 9000], [140, 70], 4, 2)])
+def test_fp16_low_tail(jo, cuda, cached, new, H, Hk, below):
+    """Every 64th key has score 0 and value 0, all others a score `below` under it and value 64: the result is
+    the tail alone, and each of its weights is small.
+
+    Bound: rounding the result (2^-11), the weights (2^-11; both together are the two-part form's too), fp32 scores,
+    exponentials and sums (2^-12), and weights held as multiples of 2^-36 of the largest: half of that for each of
+    n keys, over L = sum_j exp(s_j - max s)."""
+    D = 64
+    c = Case(cuda, cached, new, H, Hk, D, 16, "f16", seed=35, scale=0.125)
+    c.q.zero_()
+    c.q[..., 0] = 8.0
+    for b, m in enumerate(c.kv):
+        at = torch.arange(m, device=cuda)
+        blk = c.table[b].long()[at // 16]
+        top = (at % 64 == 0)[:, None]
+        c.ks[b][:, :, 0] = torch.where(top, 0.0, -below).half()
+        c.vs[b][:] = torch.where(top, 0.0, 64.0).half()[..., None]
+        c.kc[blk, at % 16], c.vc[blk, at % 16] = c.ks[b], c.vs[b]
+    for causal in (True, False):
+        for got in (c.run(jo, causal), c.run(jo, causal, max_query_len=max(new))):
+            a = 0
+            for n, m, k, v in zip(new, c.kv, c.ks, c.vs):
+                ref, _ = reference(c.q[a:a + n], k, v, causal, c.scale)
+                L = (m - n) // 64 + 1                        # at least so many keys of weight 1 in every row
+                check_rows(got[a:a + n], ref, ref * (2 * 2.0 ** -11 + 2.0 ** -12) + m * 2.0 ** -37 * 64 / L)
+                a += n
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hk", [(2, 2), (8, 2), (14, 2), (32, 1)])
+def test_few_rows_keep_their_weights(jo, cuda, H, Hk, D, dt):
+    """Requests of few rows: the weights come in two parts, so that only the result's rounding and fp32 arithmetic
+    count: |out - ref| <= u |ref| + (2^-12 + 2^-16) A + n 2^-37 max|v| / L  (A = sum_j w_j |v_j|; 2^-16: what rounding
+    the second part of a bf16 weight leaves; the last term: fp16's fixed spacing)."""
+    cached = [0, 1, 2, 3, 5, 8, 12, 20, 33, 63, 64, 100, 190, 400]
+    c = Case(cuda, cached, [1] * len(cached), H, Hk, D, 16, dt, seed=36 + H)
+    u = U[DT[dt]]
+    got = c.run(jo, max_query_len=1)
+    for b, (k, v) in enumerate(zip(c.ks, c.vs)):
+        q = c.q[b:b + 1]
+        ref, loose = reference(q, k, v, True, c.scale)
+        fixed = k.size(0) * 2.0 ** -25 * v.abs().max() if dt == "f16" else 0.0
+        s = torch.einsum("qhd,khd->qhk", q.double(), k.double().repeat_interleave(H // Hk, 1)) * c.scale
+        w = torch.softmax(s, -1)
+        A = torch.einsum("qhk,khd->qhd", w, v.double().abs().repeat_interleave(H // Hk, 1))
+        L = torch.exp(s - s.amax(-1, keepdim=True)).sum(-1, keepdim=True)
+        check_rows(got[b:b + 1], ref, u * ref.abs() + (2.0 ** -12 + 2.0 ** -16) * A + fixed * 2.0 ** -12 / L + 1e-30)
