@@ -53,10 +53,10 @@ __device__ __forceinline__ int visible(const Params& p, const Request& r, int i)
   return p.causal ? max(0, r.keys - r.n + i + 1) : r.keys;
 }
 
-// Running maxima (of scale * log2(e) * s) start here instead of at -infinity, so
-// that a step in which a row sees no key leaves exp2(0) = 1 and exp2(-inf) = 0,
-// and no NaN.
-constexpr float kNoMax = -1e30f;
+// Running maxima (of scale * log2(e) * s) start at the lowest finite number instead
+// of at -infinity, so that a step in which a row sees no key leaves exp2(0) = 1 and
+// exp2(-inf) = 0, and no NaN, while every finite score lies above it.
+constexpr float kNoMax = -3.402823466e38f;
 
 // A row's weights are exp2(x - m), where m = maximum - kUp and moves only when the
 // maximum has grown by more than kLag since: the largest weight lies in 2^kUp ..

@@ -178,3 +178,21 @@ def test_few_rows_keep_their_weights(jo, cuda, H, Hk, D, dt):
         A = torch.einsum("qhk,khd->qhd", w, v.double().abs().repeat_interleave(H // Hk, 1))
         L = torch.exp(s - s.amax(-1, keepdim=True)).sum(-1, keepdim=True)
         check_rows(got[b:b + 1], ref, u * ref.abs() + (2.0 ** -12 + 2.0 ** -16) * A + fixed * 2.0 ** -12 / L + 1e-30)
+
+
+@pytest.mark.parametrize("cached,new,H,Hk", [([100], [1], 8, 2), ([40, 9000], [2, 1], 8, 2), ([0], [1], 1, 1), ([100], [150], 4, 2),
+                                             ([9000], [64], 4, 4)])
+def test_scores_far_below_zero(jo, cuda, cached, new, H, Hk):
+    """All scores of a row are near -5e30 (bf16): the highest keys have all the weight, as anywhere else."""
+    D = 64
+    c = Case(cuda, cached, new, H, Hk, D, 16, "bf16", seed=37, scale=0.125)
+    c.q.zero_()
+    c.q[..., 0] = 2.0 ** 53
+    for b, m in enumerate(c.kv):
+        at = torch.arange(m, device=cuda)
+        c.ks[b].zero_()
+        c.ks[b][:, :, 0] = torch.where(at % 50 == 0, -(2.0 ** 52), -(2.0 ** 52) * 1.25).to(torch.bfloat16)[:, None]
+        c.kc[c.table[b].long()[at // 16], at % 16] = c.ks[b]
+    for causal in (True, False):
+        c.check(c.run(jo, causal), causal)
+        c.check(c.run(jo, causal, max_query_len=max(new)), causal)
