@@ -39,7 +39,11 @@ class SessionCache:
 
     The host keeps lengths and block lists of its own (it decides who gets blocks);
     the GPU builds tables and slots from the lengths (``paged_layout``), taking
-    blocks from the front of the free list in session order, as the host does."""
+    blocks from the front of the free list in session order, as the host does.
+
+    A step is what lies between ``begin`` and ``end``.  Its tokens and blocks become the
+    sessions' in ``end``: one that is not ended (a layer raised, a retry) is dropped by
+    the next ``begin``."""
 
     def __init__(self, layers: int, sessions: int, blocks: int, page_size: int, kv_heads: int, head_dim: int, device,
                  dtype=torch.bfloat16, max_tokens: Optional[int] = None):
@@ -53,34 +57,40 @@ class SessionCache:
         self.free: List[int] = list(range(blocks))
         self.held: List[List[int]] = [[] for _ in range(sessions)]
         self.lens = [0] * sessions
+        # of the open step: new tokens of every session, and how many blocks it gets from the free list's front
         self.new = [0] * sessions
+        self.taken = [0] * sessions
         self.layout: Optional[jo.PagedLayout] = None
 
     def begin(self, new_lens: Sequence[int], num_tokens: Optional[int] = None) -> "jo.PagedLayout":
         """Makes room for new_lens[s] tokens of every session s, side by side in the
-        step's rows; num_tokens (default: their sum) places of a padded step."""
+        step's rows; num_tokens (default: their sum) places of a padded step.  A step
+        that is still open is dropped."""
         if len(new_lens) != len(self.lens) or min(new_lens, default=0) < 0:
             raise ValueError("new_lens must have a length of 0 or more for every session")
-        need = [-(-(c + n) // self.page) - len(h) for c, n, h in zip(self.lens, new_lens, self.held)]
+        need = [self._pages(c + n) - self._pages(c) for c, n in zip(self.lens, new_lens)]
         if sum(need) > len(self.free):
             raise RuntimeError(f"{sum(need)} cache blocks are needed, {len(self.free)} are free")
-        if max(len(h) + k for h, k in zip(self.held, need)) > self.tables.size(1):
+        if max(self._pages(c + n) for c, n in zip(self.lens, new_lens)) > self.tables.size(1):
             raise RuntimeError("a session would be longer than max_tokens")
         total = sum(new_lens)
         lens = torch.tensor([self.lens, list(new_lens)], dtype=torch.int32).to(self.device)
         free = torch.tensor(self.free[:sum(need)], dtype=torch.int32).to(self.device)
         self.layout = jo.paged_layout(lens[0], lens[1], self.tables, free, self.page,
                                       total if num_tokens is None else num_tokens)
-        for h, k in zip(self.held, need):
-            h += self.free[:k]
-            del self.free[:k]
-        self.new = list(new_lens)
+        self.new, self.taken = list(new_lens), need
         return self.layout
 
     def end(self) -> None:
-        """The step's tokens are part of the sessions now."""
+        """The step's tokens and blocks are part of the sessions now."""
+        for h, k in zip(self.held, self.taken):
+            h += self.free[:k]
+            del self.free[:k]
         self.lens = [c + n for c, n in zip(self.lens, self.new)]
-        self.new = [0] * len(self.lens)
+        self.new, self.taken = [0] * len(self.lens), [0] * len(self.lens)
+
+    def _pages(self, tokens: int) -> int:
+        return -(-tokens // self.page)
 
     def release(self, session: int) -> None:
         """Ends a session; its blocks are free for others."""

@@ -1,0 +1,111 @@
+"""Bookkeeping of joyomni_stack.SessionCache without a GPU: the layout operator is
+replaced by its definition, written out request by request, and after every call the
+host's block lists are compared with what the tables then say."""
+import random
+
+import pytest
+import torch
+
+import joyomni_ops as jo
+from joyomni_stack import sessions
+
+
+def layout_on_host(cached, new, tables, free, page, num_tokens):
+    """paged_layout's definition."""
+    free = free.tolist()
+    starts, kv, slots, pos, used = [0], [], [-1] * num_tokens, [0] * num_tokens, 0
+    for b, (c, n) in enumerate(zip(cached.tolist(), new.tolist())):
+        held, want = -(-c // page), -(-(c + n) // page)
+        for j in range(held, min(want, tables.size(1))):
+            f = used + j - held
+            tables[b, j] = free[f] if f < len(free) else -1
+        used += want - held
+        for i in range(n):
+            t, block = starts[-1] + i, int(tables[b, (c + i) // page])
+            if t < num_tokens:
+                slots[t] = block * page + (c + i) % page if block >= 0 else -1
+                pos[t] = c + i
+        starts.append(starts[-1] + n)
+        kv.append(c + n)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    return jo.PagedLayout(i32(starts), i32(kv), torch.tensor(slots, dtype=torch.int64), i32(pos), i32([used]))
+
+
+@pytest.fixture(autouse=True)
+def host_layout(monkeypatch):
+    monkeypatch.setattr(sessions.jo, "paged_layout", layout_on_host)
+
+
+def cache(n, blocks=40, page=16, **kw):
+    return sessions.SessionCache(1, sessions=n, blocks=blocks, page_size=page, kv_heads=1, head_dim=8, device="cpu", **kw)
+
+
+def blocks_of(c, s, tokens):
+    return c.tables[s, :-(-tokens // c.page)].tolist()
+
+
+def check_open(c, lay, blocks=40):
+    """In a step: every token has a slot of its own, in blocks that no other session has."""
+    kv = lay.kv_lens.tolist()
+    rows = [blocks_of(c, s, n) for s, n in enumerate(kv)]
+    used = [b for r in rows for b in r]
+    assert len(set(used)) == len(used) and all(0 <= b < blocks for b in used)
+    assert kv == [x + n for x, n in zip(c.lens, c.new)]
+    t = 0
+    for s, n in enumerate(c.new):
+        for i in range(n):
+            pos = c.lens[s] + i
+            assert lay.positions[t] == pos and lay.slots[t] == rows[s][pos // c.page] * c.page + pos % c.page
+            t += 1
+    assert lay.slots[t:].tolist() == [-1] * (len(lay.slots) - t)
+
+
+def check_closed(c, blocks=40):
+    """Between steps: the tables hold the blocks that the host counts, and none is lost or given twice."""
+    for s, n in enumerate(c.lens):
+        assert blocks_of(c, s, n) == c.held[s], s
+    assert sorted(c.free + [b for h in c.held for b in h]) == list(range(blocks))
+
+
+def test_steps():
+    c = cache(3)
+    for new in ([17, 0, 40], [1, 1, 1], [0, 0, 0], [15, 30, 7]):
+        check_open(c, c.begin(new))
+        c.end()
+        check_closed(c)
+    c.release(1)
+    check_closed(c)
+    assert c.lens == [33, 0, 48]
+    check_open(c, c.begin([0, 50, 1], num_tokens=64))
+    c.end()
+    check_closed(c)
+
+
+@pytest.mark.parametrize("first,second", [([17, 0], [17, 0]), ([40, 0], [1, 20]), ([100, 3], [0, 0]), ([1, 1], [200, 0])])
+def test_a_step_begun_again(first, second):
+    """A step that was dropped leaves nothing behind: the next one has the tokens from where the last whole one ended."""
+    for before in ([0, 0], [5, 33]):
+        c = cache(2)
+        c.begin(before)
+        c.end()
+        c.begin(first)
+        check_open(c, c.begin(second))
+        c.end()
+        assert c.lens == [a + b for a, b in zip(before, second)]
+        check_closed(c)
+        check_open(c, c.begin([16, 16]))
+        c.end()
+        check_closed(c)
+
+
+def test_a_refused_step_changes_nothing():
+    c = cache(2, blocks=4, max_tokens=48)
+    c.begin([20, 5])
+    c.end()
+    for new in ([20, 30], [40, 0]):
+        with pytest.raises(RuntimeError, match="blocks are needed|max_tokens"):
+            c.begin(new)
+        check_closed(c, 4)
+    check_open(c, c.begin([12, 11]), 4)
+    c.end()
+    check_closed(c, 4)
