@@ -83,9 +83,14 @@ class SessionCache:
 
     def end(self) -> None:
         """The step's tokens and blocks are part of the sessions now."""
-        for h, k in zip(self.held, self.taken):
-            h += self.free[:k]
+        spare = []                                   # of sessions that ended within the step
+        for s, k in enumerate(self.taken):
+            if self.new[s] > 0:
+                self.held[s] += self.free[:k]
+            else:
+                spare += self.free[:k]
             del self.free[:k]
+        self.free += spare
         self.lens = [c + n for c, n in zip(self.lens, self.new)]
         self.new, self.taken = [0] * len(self.lens), [0] * len(self.lens)
 
@@ -93,10 +98,12 @@ class SessionCache:
         return -(-tokens // self.page)
 
     def release(self, session: int) -> None:
-        """Ends a session; its blocks are free for others."""
+        """Ends a session; its blocks are free for others.  Within a step, its tokens
+        of the step go with it (their rows are computed all the same)."""
         self.free += self.held[session]
         self.held[session] = []
         self.lens[session] = 0
+        self.new[session] = 0
 
     def write(self, layer: int, k, v) -> None:
         jo.paged_kv_write(k, v, *self.caches[layer], self.layout.slots)

@@ -58,3 +58,21 @@ def test_dropped_steps(cuda, dropped):
     r.cache.begin([1, 0])
     r.step([60, 30])
     r.check()
+
+
+def test_release_within_a_step(cuda):
+    """The session ends, its row of the step is computed all the same, and the others go on; its blocks are used again."""
+    r = Run(cuda, [200, 200, 200], blocks=16)
+    r.step([60, 33, 0])
+    lay = r.cache.begin([20, 20, 0])
+    x = r.rows([20, 20, 0])
+    r.cache.release(0)
+    y = r.layer.forward(x, r.cache, 0, lay)
+    r.cache.end()
+    assert rel(y[:20], eager(r.layer, r.seqs[0][:80], [80])[60:]) <= 4e-2
+    r.outs[1].append(y[20:])
+    r.outs[0] = []
+    r.seqs[0] = r.seqs[0].flip(0)
+    for new in ([1, 1, 40], [70, 30, 1], [1, 1, 1]):
+        r.step(new)
+    r.check()

@@ -109,3 +109,44 @@ def test_a_refused_step_changes_nothing():
     check_open(c, c.begin([12, 11]), 4)
     c.end()
     check_closed(c, 4)
+
+
+def test_a_session_released_within_a_step():
+    c = cache(2)
+    c.begin([40, 10])
+    c.release(0)
+    c.end()
+    assert c.lens == [0, 10]
+    check_closed(c)
+    check_open(c, c.begin([1, 20]))
+    c.end()
+    check_closed(c)
+    c.begin([30, 30])                                        # released with tokens of earlier steps, and the step dropped
+    c.release(1)
+    check_open(c, c.begin([16, 3]))
+    c.end()
+    assert c.lens == [17, 3]
+    check_closed(c)
+
+
+def test_steps_drops_and_releases_in_any_order():
+    for seed in range(200):
+        r = random.Random(seed)
+        c = cache(4, blocks=24, page=r.choice([1, 7, 16]), max_tokens=100)
+        for _ in range(30):
+            new = [r.choice([0, 0, 1, r.randrange(40)]) for _ in range(4)]
+            try:
+                lay = c.begin(new)
+            except RuntimeError:
+                c.release(r.randrange(4))
+                continue
+            check_open(c, lay, 24)
+            if r.random() < 0.3:
+                c.release(r.randrange(4))
+            if r.random() < 0.7:
+                c.end()
+                check_closed(c, 24)
+            if r.random() < 0.2:
+                c.release(r.randrange(4))
+        c.end()
+        check_closed(c, 24)
