@@ -68,12 +68,14 @@ class SessionCache:
         that is still open is dropped."""
         if len(new_lens) != len(self.lens) or min(new_lens, default=0) < 0:
             raise ValueError("new_lens must have a length of 0 or more for every session")
+        total = sum(new_lens)
+        if num_tokens is not None and num_tokens < total:
+            raise ValueError(f"num_tokens ({num_tokens}) has no room for the step's {total} tokens")
         need = [self._pages(c + n) - self._pages(c) for c, n in zip(self.lens, new_lens)]
         if sum(need) > len(self.free):
             raise RuntimeError(f"{sum(need)} cache blocks are needed, {len(self.free)} are free")
         if max(self._pages(c + n) for c, n in zip(self.lens, new_lens)) > self.tables.size(1):
             raise RuntimeError("a session would be longer than max_tokens")
-        total = sum(new_lens)
         lens = torch.tensor([self.lens, list(new_lens)], dtype=torch.int32).to(self.device)
         free = torch.tensor(self.free[:sum(need)], dtype=torch.int32).to(self.device)
         self.layout = jo.paged_layout(lens[0], lens[1], self.tables, free, self.page,

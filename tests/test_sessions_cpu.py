@@ -150,3 +150,17 @@ def test_steps_drops_and_releases_in_any_order():
                 c.release(r.randrange(4))
         c.end()
         check_closed(c, 24)
+
+
+def test_places_for_every_token():
+    """A padded step may have more places than tokens, not fewer: tokens without a place would be lost."""
+    c = cache(2)
+    c.begin([3, 4])
+    c.end()
+    with pytest.raises(ValueError, match="no room for the step's 12 tokens"):
+        c.begin([5, 7], num_tokens=11)
+    check_closed(c)
+    check_open(c, c.begin([5, 7], num_tokens=12))
+    check_open(c, c.begin([5, 7], num_tokens=30))
+    c.end()
+    assert c.lens == [8, 11]
