@@ -147,6 +147,8 @@ class SessionAttention:
     def forward(self, x, cache: SessionCache, layer: int, layout: "jo.PagedLayout", prompts: bool = False):
         """x [T, hidden], the step's rows.  prompts: every session's tokens of this
         step are all that it has, so that they need not be read back from the cache."""
+        if prompts and any(c and n for c, n in zip(cache.lens, cache.new)):
+            raise RuntimeError("prompts=True, but a session has tokens from earlier steps")
         q, k, v = self.project(x, layout.positions)
         cache.write(layer, k, v)
         o = jo.prompt_attention(q, k, v, layout.query_starts) if prompts else cache.attend(layer, q)

@@ -164,3 +164,25 @@ def test_places_for_every_token():
     check_open(c, c.begin([5, 7], num_tokens=30))
     c.end()
     assert c.lens == [8, 11]
+
+
+def bare_layer(max_positions=4096):
+    """A layer that has nothing but its tables: forward may not get as far as its weights."""
+    layer = sessions.SessionAttention.__new__(sessions.SessionAttention)
+    layer.cos = layer.sin = torch.zeros(max_positions, 4)
+    return layer
+
+
+def test_prompts_are_all_that_a_session_has():
+    c = cache(2)
+    layer, x = bare_layer(), torch.zeros(5, 8)
+    layer.project = lambda *a: pytest.fail("not refused")
+    c.begin([4, 0])
+    c.end()
+    lay = c.begin([1, 4])
+    with pytest.raises(RuntimeError, match="tokens from earlier steps"):
+        layer.forward(x, c, 0, lay, prompts=True)
+    lay = c.begin([0, 5])                                    # the other one has history, but no tokens in this step
+    layer.project = lambda *a: (_ for _ in ()).throw(KeyError("as far as the projection"))
+    with pytest.raises(KeyError, match="as far as the projection"):
+        layer.forward(x, c, 0, lay, prompts=True)
