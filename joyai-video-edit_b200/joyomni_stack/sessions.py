@@ -60,6 +60,7 @@ class SessionCache:
         # of the open step: new tokens of every session, and how many blocks it gets from the free list's front
         self.new = [0] * sessions
         self.taken = [0] * sessions
+        self.longest = 0                             # positions that its tokens reach
         self.layout: Optional[jo.PagedLayout] = None
 
     def begin(self, new_lens: Sequence[int], num_tokens: Optional[int] = None) -> "jo.PagedLayout":
@@ -81,6 +82,7 @@ class SessionCache:
         self.layout = jo.paged_layout(lens[0], lens[1], self.tables, free, self.page,
                                       total if num_tokens is None else num_tokens)
         self.new, self.taken = list(new_lens), need
+        self.longest = max((c + n for c, n in zip(self.lens, new_lens) if n), default=0)
         return self.layout
 
     def end(self) -> None:
@@ -146,7 +148,13 @@ class SessionAttention:
 
     def forward(self, x, cache: SessionCache, layer: int, layout: "jo.PagedLayout", prompts: bool = False):
         """x [T, hidden], the step's rows.  prompts: every session's tokens of this
-        step are all that it has, so that they need not be read back from the cache."""
+        step are all that it has, so that they need not be read back from the cache.
+        layout: what the cache's begin() returned for the step."""
+        # on the host: on the GPU a position past the tables would be an access out of range
+        if layout is not cache.layout:
+            raise RuntimeError("layout is not that of the cache's last begin()")
+        if cache.longest > self.cos.size(0):
+            raise RuntimeError(f"a session reaches {cache.longest} positions, the layer has {self.cos.size(0)} (max_positions)")
         if prompts and any(c and n for c, n in zip(cache.lens, cache.new)):
             raise RuntimeError("prompts=True, but a session has tokens from earlier steps")
         q, k, v = self.project(x, layout.positions)

@@ -186,3 +186,25 @@ def test_prompts_are_all_that_a_session_has():
     layer.project = lambda *a: (_ for _ in ()).throw(KeyError("as far as the projection"))
     with pytest.raises(KeyError, match="as far as the projection"):
         layer.forward(x, c, 0, lay, prompts=True)
+
+
+def test_positions_past_the_tables_are_refused():
+    """On the host, before anything is launched: on the GPU the index would be out of range."""
+    layer, x = bare_layer(max_positions=64), torch.zeros(1, 8)
+    layer.project = lambda *a: (_ for _ in ()).throw(KeyError("as far as the projection"))
+    c = cache(2)
+    with pytest.raises(KeyError):
+        layer.forward(x, c, 0, c.begin([64, 1]))
+    c.end()
+    with pytest.raises(KeyError):                            # the long session has no tokens in this step
+        layer.forward(x, c, 0, c.begin([0, 1]))
+    lay = c.begin([1, 0])
+    with pytest.raises(RuntimeError, match="reaches 65 positions, the layer has 64"):
+        layer.forward(x, c, 0, lay)
+    c.release(0)                                             # its row of the step is still there
+    with pytest.raises(RuntimeError, match="reaches 65 positions"):
+        layer.forward(x, c, 0, lay)
+    with pytest.raises(KeyError):
+        layer.forward(x, c, 0, c.begin([64, 63]))
+    with pytest.raises(RuntimeError, match="not that of the cache's last"):
+        layer.forward(x, c, 0, lay)                          # a dropped step's positions
