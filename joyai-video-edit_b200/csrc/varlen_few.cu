@@ -178,9 +178,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
     const int arow = lane & 15, acol = lane >> 4;
     const uint32_t qs = ring + C::Q0, ps = ring + C::P0;
     uint32_t it = 0;
-    // After a wait that gave up the warps skip the steps but still walk the pieces
-    // (and every one of them skips the same ones): they meet at barriers, which
-    // have no limit.
+    // After a wait that gave up the warps still go through all steps, without further
+    // waits: they meet at barriers, which have no limit.  What they compute and store
+    // from there is of no use, and the fault code is what tells; into the ring, where a
+    // late copy may still land, they write nothing.
     while (walk.next(s)) {
       const int tok0 = s.i * tpi, ntok = min(tpi, s.r.n - tok0);
       const int some = visible(p, s.r, tok0), most = visible(p, s.r, tok0 + ntok - 1);
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
             for (int i = 0; i < 4; ++i) x[t][n][i] += x2[t][n][i];
         const bool edge = (j + 1) * kKeys > some;            // some row does not see every key of this step
         int bad = 0;
-        if (edge) {
+        if (edge && ok) {
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
