@@ -276,12 +276,15 @@ int jo_paged_kv_write(const void* key, const void* value, void* key_cache, void*
  * query_starts[b] .. query_starts[b + 1] (n of them) of q [tokens, heads,
  * head_dim] and the keys 0 .. kv_lens[b] of its blocks, the new tokens' own
  * among them; row i sees keys 0 .. kv_lens[b] - n + i (causal != 0) or all.  A
- * row that sees no key is zero; rows of no request are not written.  Query
+ * row that sees no key (or only scores of -infinity) is zero; rows of no request
+ * are not written.  An infinity in a value that a row sees is infinity in its
+ * result, whatever its weight.  Query
  * head h reads key head h / (heads / kv_heads).  Places of a block that no
  * token holds are never used, whatever they contain; a table entry outside the
  * cache reads as zeros; kv_lens past table_width pages are cut there.
  * max_query_len: the largest number of new tokens of a request, as far as the
- * host knows it (it only chooses the kernels; any value gives the result).
+ * host knows it (it only chooses the kernels; any value gives the result, up to
+ * the rounding of the weights before the product with V).
  * head_dim 64 or 128; dtype JO_DTYPE_BF16/F16; page_size % 16 == 0;
  * heads / kv_heads <= 128.  row_strides: token and head strides of q, then of
  * out; cache_strides: block, token and head strides of key_cache, then of

@@ -5,7 +5,7 @@
 //
 // Request b has the query rows query_starts[b] .. query_starts[b + 1] and
 // kv_len keys; row i of its n rows sees keys 0 .. kv_len - n + i (causal) or
-// all of them.  A row that sees no key is zero.
+// all of them.  A row that sees no key, or only scores of -infinity, is zero.
 //
 // Organisation of tile_kernel (one block per SM, 384 threads).  The `group`
 // query heads that read one key head are rows of one tile: row r of a tile is
@@ -38,10 +38,10 @@
 // seen by the MMA warp (450), PV and the next QK into the place that P leaves
 // (1240), S seen (250), of which two tiles fill 2480 of 3900 cycles on the tensor
 // cores; then the power limit.  One causal prompt of 12288 tokens, 16 heads over 4
-// of 128: 557 us, 1.11 PFLOP/s; 11042 tokens over 32102 keys, 10 heads: 1.76-1.92
-// ms, 0.95-1.03 PFLOP/s.  For short ones dependent round trips: lengths, division
-// of the work, block table, first scores 5 us after the start, 4-5 us for an item
-// of one step.
+// of 128: 557-637 us, 0.97-1.11 PFLOP/s by the clocks that the limit leaves; 11042
+// tokens over 32102 keys, 10 heads: 1.70-1.92 ms, 0.95-1.07 PFLOP/s.  For short ones
+// dependent round trips: lengths, division of the work, block table, first scores 5
+// us after the start, 4-5 us for an item of one step.
 #include <math.h>
 
 #include "varlen_attention.cuh"
@@ -52,11 +52,14 @@ namespace vattn {
 constexpr int kRows = 128;               // rows of a tile
 constexpr int kKeys = 128;               // keys of a step
 constexpr int kThreads = 384;
-// Blocks work in pairs where requests have this many rows and K and V are larger
-// than L2 by half.  Pairs halve the reads of K and V and have twice the steps in
-// flight, but wait for each other: at 11042 tokens over 32102 keys the single form
-// has 1.00-1.08 PFLOP/s with 10 heads (K and V 164 MB), pairs 1.00; with 20 heads
-// (329 MB) 0.85 and 0.94.
+// Blocks work in pairs where requests have this many rows and K and V may be larger
+// than L2 by half: the host knows what the tables and the cache can hold, not the
+// lengths (kv_bytes).  Pairs halve the reads of K and V and have twice the steps in
+// flight, but wait for each other.  Single form and pairs, measured in turn: 11042
+// tokens over 32102 keys, 20 heads (K and V 329 MB) 4.05 and 3.57 ms, 10 heads (164
+// MB) 1.83 and 1.72 in one run, 1.00-1.08 and 1.00 PFLOP/s in another; 10 heads,
+// 2048 tokens over 10048 keys 115 and 118 us, over 2548 47 and 52 us, which is what a
+// chunk over a short history costs more where tables and cache are large.
 constexpr int kPairRows = 2048;
 constexpr int64_t kPairBytes = 192LL << 20;
 // Steps that an item's beginning and end cost; steps of the shortest piece; items
@@ -786,7 +789,7 @@ static int64_t workspace_bytes_for(int64_t max_keys, int head_dim) {
   return tiles_split(max_keys) || few_splits(max_keys) ? tile_workspace(head_dim) + few_workspace(head_dim) : 0;
 }
 static int64_t max_keys(const Params& p) { return p.table ? (int64_t)p.width * p.page : p.tokens; }
-// The most K and V that a call can read.
+// The most K and V that a call can read, whatever the lengths are.
 static int64_t kv_bytes(const Params& p) {
   int64_t keys = p.tokens;
   if (p.table) {

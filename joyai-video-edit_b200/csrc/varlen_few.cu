@@ -12,8 +12,8 @@
 // evenly over the blocks (varlen_attention.cuh).
 //
 // Measured, the join included: one token over 131071 cached ones (32 heads over 8
-// of 128, 537 MB) 98.5 us, 5.45 TB/s; 64 single tokens over 54480 (224 MB) 48.8 us;
-// one over 300 (14 heads over 2 of 64) 8.0 us, nearly all of it latency.
+// of 128, 537 MB) 99-102 us, 5.3-5.4 TB/s; 64 single tokens over 54480 (224 MB) 49-50
+// us; one over 300 (14 heads over 2 of 64) 8.1 us, nearly all of it latency.
 #include "varlen_attention.cuh"
 
 namespace jo {
@@ -24,8 +24,9 @@ constexpr int kKeys = 64;                // keys of a step
 constexpr int kWarps = 4;                // warps that compute
 constexpr int kThreads = 32 * (kWarps + 1);
 // Steps that an item's beginning and end cost; steps of the shortest piece; items
-// that are never cut (a join takes as long as some seven steps: 300 tokens in one
-// piece 7.6 us, in three 10.1; 4000 tokens 11.3 us, in pieces of four at least 12.4).
+// that are never cut (300 tokens, five steps: 8.1 us, in two pieces and a join 10.1;
+// 440, seven steps: 10.5 and 9.6, with the join's launch in both, since the table has
+// room for more; 4000: 11.3 us, in pieces of four at least 13.6).
 constexpr int kLead = 2, kMin = 2, kWhole = 7;
 constexpr int kBlocksPerSm = 2;
 

@@ -232,11 +232,16 @@ def paged_attention(query, key_cache, value_cache, block_tables, query_starts, k
     (int32 [B]) of its blocks in key_cache and value_cache [num_blocks, page_size,
     kv_heads, head_dim], the new tokens' own among them (paged_kv_write first);
     page_size a multiple of 16.  Row i of n sees keys 0 .. kv_lens[b] - n + i
-    (causal) or all; a row that sees none is zero.  H must be a multiple of
+    (causal) or all; a row that sees none (or only scores of -infinity) is zero.  An
+    infinity in a value that a row sees is infinity in its result, whatever its weight;
+    values that it does not see have no influence.  H must be a multiple of
     kv_heads; query head h reads key head h // (H / kv_heads).  Rows of no request
     are not written.  max_query_len: the largest number of new tokens in a
     request, if the caller knows it (1 for a decoding step): it chooses the
-    kernels and never changes what is computed.  scale defaults to
+    kernels, any value is right, and results differ by rounding: the kernel for
+    requests of up to 32 rows (new tokens times H / kv_heads) keeps 16 bits and more of
+    the weights before the product with V, the other one rounds them to query's type
+    (1.1 to 1.4 times the error of rounding the result alone).  scale defaults to
     1 / sqrt(head_dim).  workspace: varlen_attention_workspace bytes, used by one
     call at a time; by default allocated per call."""
     idx, dt = query.get_device(), query.dtype
@@ -294,7 +299,7 @@ def prompt_attention(query, key, value, seq_starts, *, causal: bool = True, scal
     are read in place); request b is rows seq_starts[b] .. seq_starts[b + 1]
     (int32 [B + 1]) of all three.  Row i sees keys 0 .. i of its own request
     (causal) or all of them.  H must be a multiple of kv_heads.  Rows of no
-    request are not written.  scale, out and workspace as in paged_attention."""
+    request are not written.  What rows see, infinities, scale, out and workspace as in paged_attention."""
     idx, dt = query.get_device(), query.dtype
     code = _DT16.get(dt)
     shape, ks = query.shape, key.shape

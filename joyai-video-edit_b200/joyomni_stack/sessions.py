@@ -11,7 +11,8 @@ grouped heads on this package's operators:
     cache <- k, v;  o = attention over the session's cache, or over the packed prompts
     x + fp8_scaled_mm(per_token_fp8(o), W_proj) + b        residual in the GEMM epilogue
 
-A step over both, with lengths and tables on the GPU throughout:
+A step over both (begin() copies the step's lengths and free blocks to the GPU and
+waits for that; what follows stays there):
 
     cache = SessionCache(layers, sessions=8, blocks=512, page_size=64, kv_heads=8, head_dim=128, device=dev)
     lay = cache.begin([77, 0, 12, 1, 1, 0, 0, 300])       # new tokens of every session
