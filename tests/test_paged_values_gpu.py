@@ -196,3 +196,27 @@ def test_scores_far_below_zero(jo, cuda, cached, new, H, Hk):
     for causal in (True, False):
         c.check(c.run(jo, causal), causal)
         c.check(c.run(jo, causal, max_query_len=max(new)), causal)
+
+
+def test_broadcast_heads(jo, cuda):
+    """Key heads and query heads that share their memory (stride 0), as expand() gives them."""
+    g = torch.Generator(device=cuda).manual_seed(38)
+    D, T = 64, 200
+    one = [torch.randn(T, 1, D, generator=g, device=cuda).to(torch.bfloat16) for _ in "qkv"]
+    q, k, v = (x.expand(T, h, D) for x, h in zip(one, (4, 2, 2)))
+    full = [x.contiguous() for x in (q, k, v)]
+    starts = starts_of([150, 50], cuda)
+    want = jo.prompt_attention(*full, starts)
+    assert torch.equal(jo.prompt_attention(q, k, v, starts), want)
+    assert torch.equal(jo.prompt_attention(full[0], k, v, starts), want)
+    assert torch.equal(jo.prompt_attention(q, *full[1:], starts), want)
+    kc, vc = (x.contiguous()[:192].view(12, 16, 1, D).expand(12, 16, 2, D) for x in one[1:])
+    table = torch.arange(12, dtype=torch.int32, device=cuda)[None]
+    for n in (1, 100):
+        a = (full[0][:n], kc.contiguous(), vc.contiguous(), table, i32([0, n], cuda), i32([190], cuda))
+        want = jo.paged_attention(*a)
+        assert torch.equal(jo.paged_attention(q[:n], kc, vc, *a[3:]), want)
+    dst = [torch.zeros(12, 16, 2, D, dtype=torch.bfloat16, device=cuda) for _ in "kv"]
+    slots = torch.arange(150, device=cuda)
+    jo.paged_kv_write(k[:150], v[:150], *dst, slots)
+    assert torch.equal(dst[0].view(-1, 2, D)[:150], full[1][:150]) and torch.equal(dst[1].view(-1, 2, D)[:150], full[2][:150])
