@@ -179,8 +179,11 @@ __device__ __noinline__ void repair_odd(const Values v, uint32_t tO, int col, in
   tmem_wait_ld();
 #pragma unroll
   for (int c = 0; c < 32; c += 8) {
+    uint32_t need = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) need |= (is_odd(__uint_as_float(o[c + i]), total) ? 1u : 0u) << i;
     float x[8];
-    odd_values<T>(v, col + c, from, common, to, limit, x);
+    odd_values<T>(v, col + c, need, from, common, to, limit, x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[c + i] = __float_as_uint(with_odd(__uint_as_float(o[c + i]), x[i], total));
   }
@@ -677,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         for (int i = 0; i < 32; i += 2)
           seen = fma2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(0.f, 0.f), seen);
         if (__any_sync(0xffffffffu, valid && l > 0.f && seen.x + seen.y != 0.f)) {
-          repair_odd<T>(Values(p, task.kfirst, task.b, task.h), tO + q, q, a * kKeys, end * kKeys, limit, l);
+          repair_odd<T>(Values(p, task.kfirst, task.b, task.h), tO + q, q, a * kKeys, end * kKeys, limit, valid ? l : 0.f);
           tmem_ld32(tO + q, o);
           tmem_wait_ld();
         }

@@ -559,31 +559,44 @@ template <typename T> __device__ __forceinline__ void add_odd(float (&sum)[8], u
   }
 }
 
-// sum[i] = sum of the values in column col + i that are not finite (0: there are
-// none) among the keys [from, min(to, limit)) of this lane's row.  A whole warp
-// calls it with rows that all see the keys below `common`, and shares those out.
+// out[i] = sum of the values in column col + i that are not finite (0: there are
+// none) among the keys [from, min(to, limit)) of this lane's row, for the columns
+// whose bit is set in `need` of any lane.  A whole warp calls it with rows that all
+// see the keys below `common`, and shares those out, until every such column has met
+// a NaN.
 template <typename T>
-__device__ __noinline__ void odd_values(const Values v, int col, int from, int common, int to, int limit, float* out) {
+__device__ __noinline__ void odd_values(const Values v, int col, uint32_t need, int from, int common, int to, int limit,
+                                        float* out) {
   const int lane = threadIdx.x & 31;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  need = __reduce_or_sync(0xffffffffu, need);
   common = min(common, to);
-#pragma unroll 4
-  for (int key = from + lane; key < common; key += 32) add_odd<T>(sum, v.at(key, col));
-  __syncwarp();
+  bool more = need != 0;
+  for (int key0 = from; more && key0 < common; key0 += 256) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (key0 + 32 * k + lane < common) add_odd<T>(sum, v.at(key0 + 32 * k + lane, col));
+    uint32_t nan = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nan |= (sum[i] != sum[i] ? 1u : 0u) << i;
+    more = (need & ~__reduce_or_sync(0xffffffffu, nan)) != 0;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+  if (more)
 #pragma unroll 1
-  for (int key = max(from, common); key < min(to, limit); ++key) add_odd<T>(sum, v.at(key, col));
+    for (int key = max(from, common); key < min(to, limit); ++key) add_odd<T>(sum, v.at(key, col));
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < 8; ++i) out[i] = sum[i];
 }
 // What a sum becomes: `odd` of its column.  total: the row's sum of weights (NaN where
 // a weight is one, 0 where it sees no key).
+__device__ __forceinline__ bool is_odd(float sum, float total) { return sum != sum && total > 0.f; }
 __device__ __forceinline__ float with_odd(float sum, float odd, float total) {
-  return sum != sum && total > 0.f && odd != 0.f ? odd : sum;
+  return is_odd(sum, total) && odd != 0.f ? odd : sum;
 }
 
 // The kernel for requests of few rows (varlen_few.cu): `rows`, the most of any

@@ -433,8 +433,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) few_kernel(const __gri
             const Values values(p, s.r.first, s.b, s.h);
 #pragma unroll
             for (int n = 0; n < NW; ++n) {
+              const uint32_t need = (is_odd(o[t][n][2 * e], sum) ? 1u : 0u) | (is_odd(o[t][n][2 * e + 1], sum) ? 2u : 0u);
               float x[8];
-              odd_values<T>(values, (warp * NW + n) * 8, s.a * kKeys, some, min(s.e * kKeys, most), limit[t][e], x);
+              odd_values<T>(values, (warp * NW + n) * 8, need << qc, s.a * kKeys, some, min(s.e * kKeys, most), limit[t][e], x);
               o[t][n][2 * e] = with_odd(o[t][n][2 * e], x[qc], sum);
               o[t][n][2 * e + 1] = with_odd(o[t][n][2 * e + 1], x[qc + 1], sum);
             }
