@@ -669,45 +669,49 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         fence_after();
       }
       const bool valid = row_tok < tpt && k_tok < task.ntok;
-      // 32 columns of O, repaired where one that should be a number or infinity is
-      // neither (one look per 32 columns: a look per row, and the whole epilogue once
-      // more, measured 48.0 us at mixed chunks against 47.4, and 47.0 without it)
-      auto load_o = [&](int q, uint32_t (&o)[32]) {
-        tmem_ld32(tO + q, o);
-        tmem_wait_ld();
-        float2 seen = make_float2(0.f, 0.f);       // NaN where one of them is not finite
+      const bool whole = task.slot < 0;
+      Slot<D, 2 * N * kRows>& slot = static_cast<Slot<D, 2 * N * kRows>*>(maps.partial)[max(task.slot, 0)];
+      const int r2 = ti * kRows + row;
+      if (!whole) slot.ml[r2] = make_float2(m, l);
+      if (has) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float2 inv2 = make_float2(inv, inv);
+        const uint32_t keep = l == 0.f ? 0u : 0xffffffffu;
+        const int row_head = row - row_tok * p.group;
+        const long long at = valid ? (long long)(task.tok + k_tok) * p.o_ts + (long long)(task.h * p.group + row_head) * p.o_hs
+                                   : -1;
+        long long to[4];                 // rows that this lane stores a piece of
 #pragma unroll
-        for (int i = 0; i < 32; i += 2)
-          seen = fma2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(0.f, 0.f), seen);
-        if (__any_sync(0xffffffffu, valid && l > 0.f && seen.x + seen.y != 0.f)) {
-          repair_odd<T>(Values(p, task.kfirst, task.b, task.h), tO + q, q, a * kKeys, end * kKeys, limit, valid ? l : 0.f);
+        for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, at, 8 * k + (lane >> 2));
+        unsigned char* buf = smem + C::OUT + warp * 2048;
+#pragma unroll 1
+        for (int q = 0; q < D; q += 32) {
+          uint32_t o[32];
           tmem_ld32(tO + q, o);
           tmem_wait_ld();
-        }
-      };
-      if (task.slot < 0) {
-        if (has) {
-          // Through shared memory, so that a warp's store covers rows of 64 bytes
-          // and not single 16-byte pieces of 32 of them.
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          const int row_head = row - row_tok * p.group;
-          const long long at = valid ? (long long)(task.tok + k_tok) * p.o_ts + (long long)(task.h * p.group + row_head) * p.o_hs
-                                     : -1;
-          long long to[4];               // rows that this lane stores a piece of
+          // 32 columns, repaired where one that should be a number or infinity is neither
+          // (ragged prompts 208-210 us, 205 without the look, 215 with loops of their own
+          // for whole items and for pieces: more code to fetch)
+          float2 seen = make_float2(0.f, 0.f);   // NaN where one of them is not finite
 #pragma unroll
-          for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, at, 8 * k + (lane >> 2));
-          unsigned char* buf = smem + C::OUT + warp * 2048;
-#pragma unroll 1
-          for (int q = 0; q < D; q += 32) {
-            uint32_t o[32];
-            load_o(q, o);
+          for (int i = 0; i < 32; i += 2)
+            seen = fma2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(0.f, 0.f), seen);
+          if (__builtin_expect(__any_sync(0xffffffffu, valid && l > 0.f && seen.x + seen.y != 0.f), 0)) {
+            repair_odd<T>(Values(p, task.kfirst, task.b, task.h), tO + q, q, a * kKeys, end * kKeys, limit, valid ? l : 0.f);
+            tmem_ld32(tO + q, o);
+            tmem_wait_ld();
+          }
+          if (whole) {
+            // Through shared memory, so that a warp's store covers rows of 64 bytes
+            // and not single 16-byte pieces of 32 of them.
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t w[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const float lo = __uint_as_float(o[8 * i + 2 * k]), hi = __uint_as_float(o[8 * i + 2 * k + 1]);
-                w[k] = l == 0.f ? 0u : pack2<T>(lo * inv, hi * inv);    // a row that sees no key is zero
+                const int c = 8 * i + 2 * k;
+                const float2 x = mul2(make_float2(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), inv2);
+                w[k] = pack2<T>(x.x, x.y) & keep;                       // a row that sees no key is zero
               }
               *reinterpret_cast<uint4*>(buf + lane * 64 + ((i ^ (lane >> 1) & 3) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -719,23 +723,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
               if (to[k] >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to[k] + q + i * 8) = w;
             }
             __syncwarp();
-          }
-        }
-      } else {
-        Slot<D, 2 * N * kRows>& slot = static_cast<Slot<D, 2 * N * kRows>*>(maps.partial)[task.slot];
-        const int r2 = ti * kRows + row;
-        slot.ml[r2] = make_float2(m, l);
-        if (has) {
-#pragma unroll 1
-          for (int q = 0; q < D; q += 32) {
-            uint32_t o[32];
-            load_o(q, o);
-            if (valid) {
+          } else if (valid) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<uint4*>(slot.o[q / 4 + i][r2]) =
-                    make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            }
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(slot.o[q / 4 + i][r2]) =
+                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
       }
