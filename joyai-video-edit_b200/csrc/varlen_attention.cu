@@ -38,7 +38,7 @@
 // seen by the MMA warp (450), PV and the next QK into the place that P leaves
 // (1240), S seen (250), of which two tiles fill 2480 of 3900 cycles on the tensor
 // cores; then the power limit.  One causal prompt of 12288 tokens, 16 heads over 4
-// of 128: 557-637 us, 0.97-1.11 PFLOP/s by the clocks that the limit leaves; 11042
+// of 128: 557-650 us, 0.95-1.11 PFLOP/s by the clocks that the limit leaves; 11042
 // tokens over 32102 keys, 10 heads: 1.70-1.92 ms, 0.95-1.07 PFLOP/s.  For short ones
 // dependent round trips: lengths, division of the work, block table, first scores 5
 // us after the start, 4-5 us for an item of one step.
